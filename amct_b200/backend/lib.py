@@ -22,6 +22,8 @@ RULE = {'released': 0, 'experimental': 1}
 PRE_NONE, PRE_MUL, PRE_DIV = 0, 1, 2
 OUT_NONE, OUT_I8, OUT_I32, OUT_PACK4, OUT_FAKE, OUT_FAKE_AWQ = range(6)
 AXIS_TENSOR, AXIS_COLUMN = 0, 1
+FP8_BLOCK = {'token': 0, 'tile': 1}
+FP8_ACT = {None: 0, 'swiglu': 1}
 DSA_DYNAMIC, DSA_LEARNED_CLIP, DSA_CLIP_RATIO, DSA_STATIC, DSA_STATIC_F32 = range(5)
 
 _lib = None
@@ -51,6 +53,7 @@ def load():
         lib.amct_minmax_workspace_bytes.argtypes = [ctypes.c_int64]
         lib.amct_minmax_noalloc_max_k.restype = ctypes.c_int64
         lib.amct_mx_tiled_scale_bytes.restype = ctypes.c_int64
+        lib.amct_moe_permute_workspace_bytes.restype = ctypes.c_int64
         lib.amct_mma_peak_ops_per_cta_step.restype = ctypes.c_int64
         _lib = lib
     return _lib

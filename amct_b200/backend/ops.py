@@ -4,7 +4,9 @@ Every function takes CUDA tensors, allocates its outputs with torch (device
 memory and streams are torch's), and enqueues the kernel on the current stream.
 Nothing here computes on the CPU: a CPU tensor raises.
 """
+import contextlib
 import ctypes
+from collections import namedtuple
 from ctypes import c_int, c_int64, c_void_p
 
 import torch
@@ -926,3 +928,298 @@ def dsa_rotate_fakequant(x, rotate=False, out_dtype=None, bits=8, symmetric=True
     _l.check(rc, 'amct_dsa_rotate_fakequant')
     COUNTERS['launches'] += 1
     return out.reshape(x.shape)
+
+
+# ---------------------------------------------------------------------------
+# FP8 with a scale for each block of 128 (the format of the FP8 checkpoints), and routed experts.  These functions
+# run on the device of their tensors, whatever device is current, and want all tensors of a call on that device.
+FP8_BLOCK_SIZE = 128
+_SAME = contextlib.nullcontext()
+
+
+def _on(*tensors):
+    """Context in which the tensors' one device is current; raises when they lie on several, or on the CPU."""
+    _need_cuda(*tensors)
+    device = None
+    for t in tensors:
+        if t is not None:
+            if device is None:
+                device = t.device
+            elif t.device != device:
+                raise _l.BackendError(f'tensors on different devices: {device} and {t.device}')
+    return _SAME if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _cdiv(a, b):
+    return (a + b - 1) // b
+
+
+def _is_codes(t):
+    return t.dtype in (torch.float8_e4m3fn, torch.uint8)
+
+
+def _rows16(codes):
+    """E4M3 codes [.., K] as the GEMMs read them: unit K stride, rows (and the rows of all leading axes together) at one
+    stride, a multiple of 16 bytes.  Anything else is copied once into such a layout."""
+    k = codes.shape[-1]
+    ld = codes.stride(-2) if codes.shape[-2] > 1 else _cdiv(k, 16) * 16
+    packed = codes.dim() == 2 or codes.shape[0] == 1 or codes.stride(0) == codes.shape[1] * ld
+    if codes.stride(-1) == 1 and ld >= k and ld % 16 == 0 and codes.data_ptr() % 16 == 0 and packed:
+        return codes, ld
+    ld = _cdiv(k, 16) * 16
+    out = torch.empty(*codes.shape[:-1], ld, dtype=torch.uint8, device=codes.device)
+    out[..., :k] = codes.view(torch.uint8)
+    return out[..., :k], ld
+
+
+def fp8_block_quant(x, block='token', act=None, pow2_scale=False):
+    """E4M3 codes and fp32 scales of x, one scale for each block of 128.
+
+    block='token' (activations): x [..., K] -> codes like x, scale [rows, ceil(K / 128)].  act='swiglu': x [..., 2 K] holds
+    gate and up halves; silu(gate) * up is quantized, codes [..., K].  block='tile' (weights): x [N, K], one scale for each
+    128 x 128 tile, [ceil(N / 128), ceil(K / 128)].  pow2_scale: scales are powers of two.
+
+    Codes are float8_e4m3fn in rows that begin at multiples of 16 bytes; token scales are stored block by block (strides
+    (1, rows)).  gemm_fp8_block reads both as they are."""
+    if block not in _l.FP8_BLOCK:
+        raise ValueError("block must be 'token' or 'tile'")
+    if act not in _l.FP8_ACT:
+        raise ValueError("act must be None or 'swiglu'")
+    tile = block == 'tile'
+    if tile and (x.dim() != 2 or act is not None):
+        raise ValueError('tile blocks take a 2-D weight and no activation function')
+    if x.dim() < 1 or (act is not None and x.shape[-1] % 2):
+        raise ValueError('swiglu needs an even number of columns: the gate half, then the up half')
+    with _on(x):
+        k = x.shape[-1] // (2 if act is not None else 1)
+        if x.numel():
+            x2, rows, _, ld = _rows2d(x)
+        else:
+            x2, rows, ld = x, (x.shape[:-1].numel() if x.dim() > 1 else 1), x.shape[-1]
+        ld_codes = _cdiv(k, 16) * 16
+        codes = torch.empty((rows, ld_codes), dtype=torch.float8_e4m3fn, device=x.device)
+        kb = _cdiv(k, FP8_BLOCK_SIZE)
+        if tile:
+            scale = torch.empty((_cdiv(rows, FP8_BLOCK_SIZE), kb), dtype=torch.float32, device=x.device)
+            stride_row, stride_k = kb, 1
+        else:
+            scale = torch.empty((kb, rows), dtype=torch.float32, device=x.device).t()
+            stride_row, stride_k = 1, rows
+        rc = _l.load().amct_fp8_block_quant(
+            _p(x2), c_int(_dt(x2)), c_int64(rows), c_int64(k), c_int64(ld), c_int(_l.FP8_BLOCK[block]), c_int(_l.FP8_ACT[act]),
+            c_int(1 if pow2_scale else 0), _p(codes), c_int64(ld_codes), _p(scale), c_int64(stride_row), c_int64(stride_k), _stream())
+        _l.check(rc, 'amct_fp8_block_quant')
+        COUNTERS['launches'] += 1
+    if ld_codes != k:
+        codes = codes[:, :k]
+    return (codes if x.dim() == 2 else codes.view(*x.shape[:-1], k) if ld_codes == k else codes.unflatten(0, x.shape[:-1]) if x.dim() > 1 else codes[0]), scale
+
+
+def _check_fp8_operands(a, a_scale, b, b_scale):
+    if not _is_codes(a) or not _is_codes(b):
+        raise ValueError('a and b must hold E4M3 codes (float8_e4m3fn or uint8)')
+    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+        raise ValueError('the scales must be float32')
+    kb = _cdiv(a.shape[1], FP8_BLOCK_SIZE)
+    if b.shape[-1] != a.shape[1]:
+        raise ValueError(f'a and b must have the same K: {tuple(a.shape)} and {tuple(b.shape)}')
+    if a.shape[1] == 0:
+        raise ValueError('K must not be zero')
+    if tuple(a_scale.shape) != (a.shape[0], kb):
+        raise ValueError(f'a_scale must be [{a.shape[0]}, {kb}], one value for each row and 128 columns')
+    if tuple(b_scale.shape) != (*b.shape[:-2], _cdiv(b.shape[-2], FP8_BLOCK_SIZE), kb):
+        raise ValueError(f'b_scale must have one value for each 128 x 128 tile of b {tuple(b.shape)}')
+
+
+def _fp8_out(out, out_dtype, m, n, device):
+    if out is None:
+        if out_dtype not in _DT:
+            raise ValueError('out_dtype must be float32, float16 or bfloat16')
+        return torch.empty((m, n), dtype=out_dtype, device=device)
+    if out.dtype not in _DT or tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+        raise ValueError(f'out must be float32 / float16 / bfloat16 [{m}, {n}] with unit inner stride')
+    return out
+
+
+def gemm_fp8_block(a, a_scale, b_nk, b_scale, bias=None, out_dtype=torch.bfloat16, out=None, status=None):
+    """a [M, K] x b_nk [N, K] -> [M, N] for E4M3 codes (float8_e4m3fn or uint8) with a scale for each block of 128:
+    a_scale fp32 [M, ceil(K / 128)], b_scale fp32 [ceil(N / 128), ceil(K / 128)], any strides.  bias [N] in fp32 / fp16 / bf16.
+    fp32 accumulation, rounded once to out_dtype.  No gradient (deploy path)."""
+    if a.dim() != 2 or b_nk.dim() != 2:
+        raise ValueError('a must be [M, K] and b_nk [N, K]')
+    _check_fp8_operands(a, a_scale, b_nk, b_scale)
+    m, k = a.shape
+    n = b_nk.shape[0]
+    bk = 0
+    if bias is not None:
+        if bias.numel() != n or bias.dtype not in _DT:
+            raise ValueError(f'bias must hold {n} values in float32, float16 or bfloat16')
+        bias = bias.reshape(-1).contiguous()
+        bk = _BIAS_KIND[bias.dtype]
+    with _on(a, a_scale, b_nk, b_scale, bias, out, status):
+        out = _fp8_out(out, out_dtype, m, n, a.device)
+        if m == 0 or n == 0:
+            return out
+        a, ld_a = _rows16(a)
+        b_nk, ld_b = _rows16(b_nk)
+        prof = _prof_begin()
+        rc = _l.load().amct_gemm_fp8_block(
+            _p(a), _p(a_scale), c_int64(a_scale.stride(0)), c_int64(a_scale.stride(1)), _p(b_nk), _p(b_scale),
+            c_int64(b_scale.stride(0)), c_int64(b_scale.stride(1)), c_int64(m), c_int64(n), c_int64(k), c_int64(ld_a), c_int64(ld_b),
+            _p(bias), c_int(bk), _p(out), c_int(_OUT_KIND[out.dtype]), c_int64(out.stride(0) if m > 1 else n), _p(status), _stream())
+        _l.check(rc, 'amct_gemm_fp8_block')
+        COUNTERS['launches'] += 1
+        _prof_end(prof, 2 * m * n * k)
+    return out
+
+
+def gemm_fp8_block_grouped(a, a_scale, offsets, b_enk, b_scale, out_dtype=torch.bfloat16, out=None, status=None):
+    """gemm_fp8_block for rows sorted by expert: rows [offsets[e], offsets[e + 1]) of a meet b_enk[e].
+
+    offsets: int32 [E + 1] on the device (moe_permute's); b_enk [E, N, K], b_scale [E, ceil(N / 128), ceil(K / 128)].  Rows of
+    the result that belong to no expert (from offsets[E] on) are left as they were in `out`; without `out` they hold
+    whatever the allocation held."""
+    if a.dim() != 2 or b_enk.dim() != 3:
+        raise ValueError('a must be [M, K] and b_enk [E, N, K]')
+    _check_fp8_operands(a, a_scale, b_enk, b_scale)
+    m, k = a.shape
+    experts, n = b_enk.shape[:2]
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() != experts + 1:
+        raise ValueError(f'offsets must be int32 [{experts + 1}]')
+    if experts == 0:
+        raise ValueError('at least one expert')
+    with _on(a, a_scale, offsets, b_enk, b_scale, out, status):
+        out = _fp8_out(out, out_dtype, m, n, a.device)
+        if m == 0 or n == 0:
+            return out
+        offsets = offsets.contiguous()
+        a, ld_a = _rows16(a)
+        b_enk, ld_b = _rows16(b_enk)
+        prof = _prof_begin()
+        rc = _l.load().amct_gemm_fp8_block_grouped(
+            _p(a), _p(a_scale), c_int64(a_scale.stride(0)), c_int64(a_scale.stride(1)), _p(offsets), c_int(experts),
+            _p(b_enk), _p(b_scale), c_int64(b_scale.stride(0)), c_int64(b_scale.stride(1)), c_int64(b_scale.stride(2)),
+            c_int64(m), c_int64(n), c_int64(k), c_int64(ld_a), c_int64(ld_b), _p(out), c_int(_OUT_KIND[out.dtype]),
+            c_int64(out.stride(0) if m > 1 else n), _p(status), _stream())
+        _l.check(rc, 'amct_gemm_fp8_block_grouped')
+        COUNTERS['launches'] += 1
+        _prof_end(prof, 2 * m * n * k)
+    return out
+
+
+#: Where moe_permute put the assignments: row_map int32 [T, topk] (the row of each, -1: held elsewhere), offsets int32
+#: [E + 1] (first row of every expert; the last entry is the number of rows in use).
+MoePlan = namedtuple('MoePlan', ['row_map', 'offsets'])
+MOE_FEW_ASSIGNMENTS = 1024
+
+
+def _strided_rows(t):
+    """[R, C] with unit inner stride and rows that do not overlap (copied otherwise), and the row stride."""
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def moe_permute(x, expert_ids, num_experts, scales=None):
+    """Tokens sorted by expert: rows[plan.row_map[t, j]] = x[t] for every (t, j) whose expert number is in [0, num_experts).
+
+    x [T, H] of any 1-, 2- or 4-byte type (fp32 / fp16 / bf16 hidden states, E4M3 or INT8 codes), expert_ids int32 / int64
+    [T, topk], scales None or fp32 [T, C], permuted along.  Returns (rows [T * topk, H], row_scales or None, plan); the
+    order within an expert is that of the flattened ids, and rows that no assignment has (from plan.offsets[-1] on) are
+    zero.  Rows of one-byte codes begin at multiples of 16 bytes and row_scales are stored column by column, as
+    gemm_fp8_block_grouped reads them.  Differentiable form: experimental...deepseek_v3_2.experts.permute_tokens."""
+    if x.dim() != 2 or expert_ids.dim() != 2 or expert_ids.shape[0] != x.shape[0] or expert_ids.shape[1] == 0:
+        raise ValueError('x must be [T, H] and expert_ids [T, topk] with topk > 0')
+    if expert_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError('expert_ids must be int32 or int64')
+    if x.element_size() not in (1, 2, 4):
+        raise ValueError(f'elements of 1, 2 or 4 bytes only, not {x.dtype}')
+    if scales is not None and (scales.dtype != torch.float32 or scales.dim() != 2 or scales.shape[0] != x.shape[0]):
+        raise ValueError('scales must be float32 [T, C]')
+    tokens, hidden = x.shape
+    topk = expert_ids.shape[1]
+    n = tokens * topk
+    with _on(x, expert_ids, scales):
+        dev = x.device
+        x, ld_x = _strided_rows(x)
+        expert_ids = expert_ids.contiguous()
+        ld_rows = _cdiv(hidden, 16) * 16 if x.element_size() == 1 else hidden
+        rows = torch.empty((n, ld_rows), dtype=x.dtype, device=dev)
+        row_map = torch.empty((tokens, topk), dtype=torch.int32, device=dev)
+        offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+        row_scales = None
+        cols = 0
+        if scales is not None:
+            cols = scales.shape[1]
+            row_scales = torch.empty((cols, n), dtype=torch.float32, device=dev).t()
+        L = _l.load()
+        ws = None
+        if n > MOE_FEW_ASSIGNMENTS:
+            ws = torch.empty(max(4, L.amct_moe_permute_workspace_bytes(c_int64(n), c_int(num_experts))), dtype=torch.uint8, device=dev)
+        rc = L.amct_moe_permute(
+            _p(x), c_int(x.element_size()), c_int64(tokens), c_int64(hidden), c_int64(ld_x), _p(expert_ids),
+            c_int(1 if expert_ids.dtype == torch.int64 else 0), c_int(topk), c_int(num_experts), _p(scales), c_int64(cols),
+            c_int64(scales.stride(0) if cols else 0), c_int64(scales.stride(1) if cols else 0), _p(rows), c_int64(ld_rows),
+            _p(row_scales), c_int64(1), c_int64(n), _p(row_map), _p(offsets), _p(ws), _stream())
+        _l.check(rc, 'amct_moe_permute')
+        COUNTERS['launches'] += 1 if n <= MOE_FEW_ASSIGNMENTS else 3
+    return rows if ld_rows == hidden else rows[:, :hidden], row_scales, MoePlan(row_map, offsets)
+
+
+def _check_moe_plan(rows, plan, weights):
+    if rows.dim() != 2 or plan.row_map.dim() != 2 or plan.row_map.dtype != torch.int32:
+        raise ValueError('rows must be [R, H] and plan.row_map int32 [T, topk]')
+    if rows.shape[0] != plan.row_map.numel():
+        raise ValueError(f'rows must have one row for each of the {plan.row_map.numel()} assignments')
+    if weights is not None and (weights.shape != plan.row_map.shape or weights.dtype not in _DT):
+        raise ValueError('weights must be float32 / float16 / bfloat16 of the shape of the expert ids')
+
+
+def moe_unpermute(rows, plan, weights=None):
+    """out[t] = sum_j weights[t, j] * rows[plan.row_map[t, j]] (fp32 sum in the order of j, rounded once to rows' dtype) over
+    the assignments that have a row.  weights None: ones, the gradient of moe_permute.  Returns [T, H]."""
+    _check_moe_plan(rows, plan, weights)
+    tokens, topk = plan.row_map.shape
+    hidden = rows.shape[1]
+    with _on(rows, plan.row_map, weights):
+        out = torch.empty((tokens, hidden), dtype=rows.dtype, device=rows.device)
+        if out.numel() == 0:
+            return out
+        rows, ld = _strided_rows(rows)
+        row_map = plan.row_map.contiguous()
+        weights = None if weights is None else weights.contiguous()
+        rc = _l.load().amct_moe_unpermute(
+            _p(rows), c_int(_dt(rows)), c_int64(rows.shape[0]), c_int64(tokens), c_int(topk), c_int64(hidden), c_int64(ld),
+            _p(row_map), _p(weights), c_int(0 if weights is None else _dt(weights)), _p(out), c_int64(hidden), _stream())
+        _l.check(rc, 'amct_moe_unpermute')
+        COUNTERS['launches'] += 1
+    return out
+
+
+def moe_unpermute_backward(grad_out, rows, plan, weights=None, want_rows=True, want_weights=True):
+    """(grad_rows, grad_weights) of moe_unpermute for the gradient grad_out [T, H]; what is not wanted is None.  Rows that no
+    assignment has get zero gradient.  rows is needed for grad_weights only."""
+    _check_moe_plan(rows, plan, weights)
+    tokens, topk = plan.row_map.shape
+    hidden = rows.shape[1]
+    want_weights = want_weights and weights is not None
+    if tuple(grad_out.shape) != (tokens, hidden) or grad_out.dtype != rows.dtype:
+        raise ValueError(f'grad_out must be [{tokens}, {hidden}] in the dtype of rows')
+    with _on(grad_out, rows, plan.row_map, plan.offsets, weights):
+        dev = rows.device
+        grad_rows = torch.empty((rows.shape[0], hidden), dtype=rows.dtype, device=dev) if want_rows else None
+        grad_weights = torch.empty((tokens, topk), dtype=weights.dtype, device=dev) if want_weights else None
+        if tokens == 0 or not (want_rows or want_weights):
+            return grad_rows, grad_weights
+        grad_out, ld_g = _strided_rows(grad_out)
+        rows, ld = _strided_rows(rows)
+        row_map = plan.row_map.contiguous()
+        weights = None if weights is None else weights.contiguous()
+        used = plan.offsets[-1:]
+        rc = _l.load().amct_moe_unpermute_backward(
+            _p(grad_out), _p(rows), c_int(_dt(rows)), c_int64(rows.shape[0]), c_int64(tokens), c_int(topk), c_int64(hidden),
+            c_int64(ld_g), c_int64(ld), _p(row_map), _p(used), _p(weights), c_int(0 if weights is None else _dt(weights)),
+            _p(grad_rows), c_int64(hidden), _p(grad_weights), _stream())
+        _l.check(rc, 'amct_moe_unpermute_backward')
+        COUNTERS['launches'] += 1
+    return grad_rows, grad_weights

@@ -1,0 +1,733 @@
+// The product of E4M3 operands with one fp32 scale for each block of 128 (sm_100a), dense and for rows sorted by expert:
+//
+//   C[m, n] = sum over kb of sa[m, kb] * sb[n / 128, kb] * dot(A[m, 128 kb ..], B[n, 128 kb ..])   (+ bias[n])
+//
+// A [rows, K] and B [N, K] (or [experts, N, K]) are E4M3 bytes, K contiguous; sa is fp32 with one value for each row and
+// 128 columns, sb one for each 128 x 128 tile: the checkpoint format that
+// amct_pytorch/experimental/quantization/DeepSeekV3.2/deploy.py:48-90 dequantizes.  The scales are arbitrary fp32
+// numbers, so they cannot ride in the MMA (its block scales are powers of two): the tensor core sums 128 products into
+// tensor memory, and the epilogue warps fold that partial sum, times sa * sb, into fp32 registers.  A tensor-memory
+// buffer holds ONE K block; there are several, so that the MMAs of the next blocks run while a block is folded in.
+//
+// Two kernels, both with a TMA producer warp, one MMA-issuing thread and epilogue warps:
+//   wide    128 rows of A x 256 columns, persistent.  A lane owns a row, so sa * sb is one number per K block and the fold
+//           is one FMA per element: 128 x 256 FMAs and as many tensor-memory reads against 512 cycles of MMA.
+//   narrow  for few rows (a decode batch): the weight is the 128-row MMA operand, 16 to 128 tokens are its columns.  Bound
+//           by the weight's bytes; K is split over a thread-block cluster whose CTAs add their partial sums through
+//           distributed shared memory in rank order, so a small weight still occupies every SM and results repeat.
+// Grouped: offsets [experts + 1] on the device say which rows belong to which expert.  Every CTA builds the table of
+// row tiles from them; a tile may read rows of the next expert (it never stores them).  Offsets that are out of
+// range or not ascending are clamped to a running maximum within [0, rows]: no access depends on their values.
+//
+// K need not be a multiple of 128: the tensor maps end at K and the rest of the last block reads as zero.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "tc05.cuh"
+
+namespace amct {
+namespace f8g {
+
+constexpr int kBlock = 128;                     // rows of an MMA tile, and bytes of K per pipeline stage
+constexpr int kMaxExperts = 1024;
+
+struct Params {
+  int64_t m, n, k;
+  const float* sa;
+  int64_t sa_row, sa_k;        // strides in elements
+  const float* sb;
+  int64_t sb_expert, sb_row, sb_k;
+  const void* bias;
+  int bias_kind;               // AMCT_BIAS_NONE / F32 / F16 / BF16
+  void* out;
+  int out_kind;                // AMCT_GEMM_OUT_F32 / F16 / BF16
+  int64_t ld_out;
+  const int* offsets;          // [experts + 1], or null: one group of m rows
+  int experts;
+  int group_m;                 // wide kernel, dense: row tiles per rasterisation group
+  int* status;
+};
+
+// ---------------------------------------------------------------------------------------------- row tiles of the groups
+struct GroupTable {
+  int bound[kMaxExperts + 1];  // first row of every group, made ascending
+  int first[kMaxExperts + 1];  // first row tile of every group
+};
+
+// Whole block; THREADS a multiple of 32.
+template <int THREADS, int TILE>
+__device__ __forceinline__ void build_groups(const Params& p, GroupTable& g) {
+  const int n = p.experts + 1;
+  const int rows = (int)p.m;
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const int v = __ldg(p.offsets + i);
+    g.bound[i] = v < 0 ? 0 : v > rows ? rows : v;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, per = (n + 31) / 32;
+    const int lo = lane * per < n ? lane * per : n, hi = lo + per < n ? lo + per : n;
+    int top = 0;
+    for (int i = lo; i < hi; ++i) top = max(top, g.bound[i]);
+    int incl = top;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl = max(incl, v);
+    }
+    int run = __shfl_up_sync(0xffffffffu, incl, 1);
+    if (lane == 0) run = 0;
+    for (int i = lo; i < hi; ++i) {
+      run = max(run, g.bound[i]);
+      g.bound[i] = run;
+    }
+    __syncwarp();
+    int sum = 0;
+    for (int i = lo; i < hi; ++i) sum += i < p.experts ? (g.bound[i + 1] - g.bound[i] + TILE - 1) / TILE : 0;
+    incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    int at = incl - sum;
+    for (int i = lo; i < hi; ++i) {
+      g.first[i] = at;
+      at += i < p.experts ? (g.bound[i + 1] - g.bound[i] + TILE - 1) / TILE : 0;
+    }
+  }
+  __syncthreads();
+}
+
+struct Tile {
+  int64_t row0, row_end;       // rows [row0, min(row0 + tile, row_end)) are this tile's
+  int64_t tn;                  // column tile
+  int expert;
+};
+
+// Grouped: all tiles of a group lie together, row tiles fastest, so that CTAs running at one time share its weight.
+template <int TILE>
+__device__ __forceinline__ Tile group_tile(const Params& p, const GroupTable& g, int64_t tile, int64_t tiles_n) {
+  const int want = (int)(tile / tiles_n);
+  int lo = 0, hi = p.experts;                    // first[lo] <= want < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (g.first[mid] <= want) lo = mid; else hi = mid;
+  }
+  Tile t;
+  t.expert = lo;
+  const int64_t rel = tile - (int64_t)g.first[lo] * tiles_n;
+  const int64_t mt = g.first[lo + 1] - g.first[lo];
+  t.tn = rel / mt;
+  t.row0 = g.bound[lo] + (rel - t.tn * mt) * TILE;
+  t.row_end = g.bound[lo + 1];
+  return t;
+}
+
+template <int TILE>
+__device__ __forceinline__ Tile dense_tile(const Params& p, int64_t tile, int64_t tiles_m, int64_t tiles_n) {
+  const int64_t per_group = (int64_t)p.group_m * tiles_n;
+  const int64_t g = tile / per_group, r = tile - g * per_group;
+  const int64_t m0 = g * p.group_m;
+  const int64_t gm = (tiles_m - m0) < p.group_m ? (tiles_m - m0) : p.group_m;
+  Tile t;
+  t.tn = r / gm;
+  t.row0 = (m0 + (r - t.tn * gm)) * TILE;
+  t.row_end = p.m;
+  t.expert = 0;
+  return t;
+}
+
+// a bounded wait of a whole warp: all of its lanes go on, or none
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, tc05::mbar_wait(bar, parity, abort_flag));
+}
+
+__device__ __forceinline__ float bias_at(const Params& p, int64_t n) {
+  switch (p.bias_kind) {
+    case AMCT_BIAS_F32: return reinterpret_cast<const float*>(p.bias)[n];
+    case AMCT_BIAS_F16: return __half2float(reinterpret_cast<const __half*>(p.bias)[n]);
+    case AMCT_BIAS_BF16: return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[n]);
+  }
+  return -0.f;                                   // x + (-0) is x for every x
+}
+
+// ---------------------------------------------------------------------------------------------- wide kernel
+constexpr int kWideN = 256, kWideStages = 4, kWideEpiWarps = 8, kWideThreads = 64 + 32 * kWideEpiWarps;
+constexpr int kWideA = kBlock * kBlock, kWideB = kWideN * kBlock, kWideStageBytes = kWideA + kWideB;
+
+struct __align__(1024) WideSmem {
+  uint8_t tiles[kWideStages][kWideStageBytes];
+  GroupTable groups;
+  uint64_t full[kWideStages], empty[kWideStages], tmem_full[2], tmem_empty[2];
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+// 128 columns of one row
+__device__ __forceinline__ void store_row128(const Params& p, int64_t row, int64_t n0, float (&acc)[128]) {
+  const int64_t off = row * p.ld_out + n0;
+#pragma unroll
+  for (int c0 = 0; c0 < 128; c0 += 32) {
+    const int64_t left = p.n - (n0 + c0);
+    if (left <= 0) break;
+    float y[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = acc[c0 + j];
+    if (p.bias_kind != AMCT_BIAS_NONE) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], j < left ? bias_at(p, n0 + c0 + j) : 0.f);
+    }
+    if (p.out_kind == AMCT_GEMM_OUT_F32) {
+      float* o = reinterpret_cast<float*>(p.out) + off + c0;
+      if (left >= 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(o + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) if (j < left) o[j] = y[j];
+      }
+    } else {
+      uint32_t h[16];
+      epi_pack16(y, p.out_kind == AMCT_GEMM_OUT_BF16, h);
+      uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + off + c0;
+      if (left >= 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(o + 2 * j) = make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) if (j < left) o[j] = (uint16_t)(h[j >> 1] >> (16 * (j & 1)));
+      }
+    }
+  }
+}
+
+template <bool GROUPED>
+__global__ void __launch_bounds__(kWideThreads, 1)
+gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  WideSmem& s = *reinterpret_cast<WideSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_kb = (int)((p.k + kBlock - 1) / kBlock);
+  const int64_t tiles_n = (p.n + kWideN - 1) / kWideN;
+  const int64_t tiles_m = (p.m + kBlock - 1) / kBlock;
+
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    for (int i = 0; i < kWideStages; ++i) { tc05::mbar_init(tc05::smem_u32(&s.full[i]), 1); tc05::mbar_init(tc05::smem_u32(&s.empty[i]), 1); }
+    for (int i = 0; i < 2; ++i) { tc05::mbar_init(tc05::smem_u32(&s.tmem_full[i]), 1); tc05::mbar_init(tc05::smem_u32(&s.tmem_empty[i]), kWideEpiWarps); }
+    tc05::fence_barrier_init();
+    tc05::prefetch_tmap(&tma_a);
+    tc05::prefetch_tmap(&tma_b);
+  }
+  if (warp == 1) {
+    tc05::tmem_alloc(tc05::smem_u32(&s.tmem_base), 512);
+    tc05::tmem_relinquish();
+  }
+  if (GROUPED) build_groups<kWideThreads, kBlock>(p, s.groups);
+  tc05::fence_before_sync();
+  __syncthreads();
+  tc05::fence_after_sync();
+  const uint32_t tmem_base = s.tmem_base;
+  volatile int* abort_flag = &s.abort_flag;
+  const int64_t num_tiles = GROUPED ? (int64_t)s.groups.first[p.experts] * tiles_n : tiles_m * tiles_n;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (tc05::elect_one()) {
+      uint32_t stage = 0, phase = 0;
+      bool alive = true;
+      for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+        const Tile t = GROUPED ? group_tile<kBlock>(p, s.groups, tile, tiles_n) : dense_tile<kBlock>(p, tile, tiles_m, tiles_n);
+        const int row_b = (int)(t.expert * p.n + t.tn * kWideN);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!tc05::mbar_wait(tc05::smem_u32(&s.empty[stage]), phase ^ 1, abort_flag)) { alive = false; break; }
+          const uint32_t bar = tc05::smem_u32(&s.full[stage]);
+          tc05::mbar_expect_tx(bar, kWideStageBytes);
+          const uint32_t dst = tc05::smem_u32(&s.tiles[stage][0]);
+          tc05::tma_load_2d(dst, &tma_a, bar, kb * kBlock, (int)t.row0);
+          tc05::tma_load_2d(dst + kWideA, &tma_b, bar, kb * kBlock, row_b);
+          if (++stage == kWideStages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer: one tensor-memory buffer per K block
+    if (tc05::elect_one()) {
+      constexpr uint32_t idesc = tc05::make_idesc(1, 0, 0, kBlock, kWideN);
+      uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
+      bool alive = true;
+      for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!tc05::mbar_wait(tc05::smem_u32(&s.tmem_empty[buf]), buf_phase ^ 1, abort_flag)) { alive = false; break; }
+          if (!tc05::mbar_wait(tc05::smem_u32(&s.full[stage]), phase, abort_flag)) { alive = false; break; }
+          tc05::fence_after_sync();
+          const uint32_t a0 = tc05::smem_u32(&s.tiles[stage][0]);
+          const uint32_t b0 = a0 + kWideA;
+#pragma unroll
+          for (int ks = 0; ks < kBlock / 32; ++ks)
+            tc05::umma_f8(tmem_base + buf * kWideN, tc05::smem_desc_sw128(a0 + ks * 32), tc05::smem_desc_sw128(b0 + ks * 32), idesc, ks > 0);
+          tc05::umma_commit(tc05::smem_u32(&s.empty[stage]));
+          tc05::umma_commit(tc05::smem_u32(&s.tmem_full[buf]));
+          if (++stage == kWideStages) { stage = 0; phase ^= 1; }
+          if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ fold and store: 32 rows x 128 columns per warp
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    uint32_t buf = 0, buf_phase = 0;
+    bool alive = true;
+    for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+      const Tile t = GROUPED ? group_tile<kBlock>(p, s.groups, tile, tiles_n) : dense_tile<kBlock>(p, tile, tiles_m, tiles_n);
+      const int64_t row = t.row0 + quarter * 32 + lane;
+      const int64_t n0 = t.tn * kWideN + half * 128;
+      const bool row_in = row < t.row_end, cols_in = n0 < p.n;
+      const float* sa = p.sa + (row_in ? row : t.row0) * p.sa_row;
+      const float* sb = p.sb + t.expert * p.sb_expert + (cols_in ? n0 / kBlock : 0) * p.sb_row;
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      float next_a = __ldg(sa), next_b = __ldg(sb);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        const float f = __fmul_rn(next_a, next_b);
+        if (kb + 1 < num_kb) {                   // the next block's scales are on their way while this one is folded
+          next_a = __ldg(sa + (kb + 1) * p.sa_k);
+          next_b = __ldg(sb + (kb + 1) * p.sb_k);
+        }
+        if (!warp_wait(tc05::smem_u32(&s.tmem_full[buf]), buf_phase, abort_flag)) { alive = false; break; }
+        tc05::fence_after_sync();
+        const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * kWideN + half * 128;
+        uint32_t r[2][32];
+        tc05::tmem_ld_32x32(t_row, r[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tc05::tmem_ld_wait(r[c & 1]);
+          if (c < 3) tc05::tmem_ld_32x32(t_row + (c + 1) * 32, r[(c + 1) & 1]);
+          else {
+            tc05::fence_before_sync();           // everything read: the buffer goes back before the last folds
+            __syncwarp();
+            if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&s.tmem_empty[buf]));
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c * 32 + j] = __fmaf_rn(__uint_as_float(r[c & 1][j]), f, acc[c * 32 + j]);
+        }
+        if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+      }
+      if (alive && row_in && cols_in) store_row128(p, row, n0, acc);
+      __syncwarp();
+    }
+  }
+
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, 2);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);      // let copies and MMAs in flight land
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc05::fence_after_sync();
+    tc05::tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- narrow kernel
+constexpr int kNarrowThreads = 192;
+constexpr int kNarrowBufs = 4;
+
+// Up to 64 tokens two CTAs share an SM (about 110 KB of shared memory and 168 registers a thread each); 128 tokens need
+// their accumulators' registers and take an SM alone.
+template <int NT> constexpr int narrow_ctas() { return NT <= 64 ? 2 : 1; }
+template <int NT> constexpr int narrow_stages() { return NT <= 32 ? 5 : NT <= 64 ? 4 : 6; }
+
+template <int NT>
+struct __align__(1024) NarrowSmem {
+  static constexpr int kStageBytes = (kBlock + NT) * kBlock;
+  uint8_t tiles[narrow_stages<NT>()][kStageBytes];    // the K loop's ring, afterwards this CTA's partial sums [NT][128]
+  float factor[4][2][NT];                             // per epilogue warp: sa * sb of a K block
+  GroupTable groups;
+  uint64_t full[narrow_stages<NT>()], empty[narrow_stages<NT>()], tmem_full[kNarrowBufs], tmem_empty[kNarrowBufs];
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store_one(const Params& p, int64_t row, int64_t n, float v) {
+  const int64_t off = row * p.ld_out + n;
+  switch (p.out_kind) {
+    case AMCT_GEMM_OUT_F32: reinterpret_cast<float*>(p.out)[off] = v; break;
+    case AMCT_GEMM_OUT_F16: reinterpret_cast<__half*>(p.out)[off] = __float2half_rn(v); break;
+    default: reinterpret_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
+  }
+}
+
+// `COLS` (16, or a multiple of 32) consecutive tensor-memory columns of this lane's row
+template <int COLS>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[COLS]) {
+  if constexpr (COLS == 16) {
+    tc05::tmem_ld_32x16(taddr, r);
+    tc05::tmem_ld_wait(r);
+  } else {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32) tc05::tmem_ld_32x32(taddr + c, *reinterpret_cast<uint32_t(*)[32]>(&r[c]));
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32) tc05::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(&r[c]));
+  }
+}
+
+// Grid: splits CTAs (one cluster) for each tile.  CTA `rank` of a cluster takes the K blocks
+// [rank * num_kb / splits, (rank + 1) * num_kb / splits).
+template <int NT, bool GROUPED>
+__global__ void __launch_bounds__(kNarrowThreads, narrow_ctas<NT>())
+gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x, Params p, int splits) {
+  constexpr int kStages = narrow_stages<NT>();
+  constexpr uint32_t kTmemCols = NT * kNarrowBufs < 32 ? 32 : NT * kNarrowBufs;
+  extern __shared__ uint8_t smem_raw[];
+  NarrowSmem<NT>& s = *reinterpret_cast<NarrowSmem<NT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = splits > 1 ? tc05::cluster_ctarank() : 0;
+  const int num_kb_all = (int)((p.k + kBlock - 1) / kBlock);
+  const int kb_lo = (int)((int64_t)num_kb_all * rank / splits), kb_hi = (int)((int64_t)num_kb_all * (rank + 1) / splits);
+  const int64_t tiles_n = (p.n + kBlock - 1) / kBlock;
+  const int64_t tile = blockIdx.x / splits;
+
+  Tile t;
+  if (GROUPED) {
+    build_groups<kNarrowThreads, NT>(p, s.groups);
+    if (tile >= (int64_t)s.groups.first[p.experts] * tiles_n) return;      // the whole cluster leaves
+    t = group_tile<NT>(p, s.groups, tile, tiles_n);
+  } else {
+    const int64_t tiles_m = (p.m + NT - 1) / NT;
+    t.tn = tile / tiles_m;                       // row tiles fastest: they share a slice of the weight
+    t.row0 = (tile - t.tn * tiles_m) * NT;
+    t.row_end = p.m;
+    t.expert = 0;
+  }
+  const int64_t n0 = t.tn * kBlock;
+
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    for (int i = 0; i < kStages; ++i) { tc05::mbar_init(tc05::smem_u32(&s.full[i]), 1); tc05::mbar_init(tc05::smem_u32(&s.empty[i]), 1); }
+    for (int i = 0; i < kNarrowBufs; ++i) { tc05::mbar_init(tc05::smem_u32(&s.tmem_full[i]), 1); tc05::mbar_init(tc05::smem_u32(&s.tmem_empty[i]), 4); }
+    tc05::fence_barrier_init();
+    tc05::prefetch_tmap(&tma_w);
+    tc05::prefetch_tmap(&tma_x);
+  }
+  if (warp == 1) {
+    tc05::tmem_alloc(tc05::smem_u32(&s.tmem_base), kTmemCols);
+    tc05::tmem_relinquish();
+  }
+  tc05::fence_before_sync();
+  __syncthreads();
+  tc05::fence_after_sync();
+  const uint32_t tmem_base = s.tmem_base;
+  volatile int* abort_flag = &s.abort_flag;
+  float acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = 0.f;
+
+  if (warp == 0) {
+    if (tc05::elect_one()) {
+      uint32_t stage = 0, phase = 0;
+      const int row_w = (int)(t.expert * p.n + n0);
+      for (int kb = kb_lo; kb < kb_hi; ++kb) {
+        if (!tc05::mbar_wait(tc05::smem_u32(&s.empty[stage]), phase ^ 1, abort_flag)) break;
+        const uint32_t bar = tc05::smem_u32(&s.full[stage]);
+        tc05::mbar_expect_tx(bar, NarrowSmem<NT>::kStageBytes);
+        const uint32_t dst = tc05::smem_u32(&s.tiles[stage][0]);
+        tc05::tma_load_2d(dst, &tma_w, bar, kb * kBlock, row_w);
+        tc05::tma_load_2d(dst + kBlock * kBlock, &tma_x, bar, kb * kBlock, (int)t.row0);
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (tc05::elect_one()) {
+      constexpr uint32_t idesc = tc05::make_idesc(1, 0, 0, kBlock, NT);
+      uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
+      for (int kb = kb_lo; kb < kb_hi; ++kb) {
+        if (!tc05::mbar_wait(tc05::smem_u32(&s.tmem_empty[buf]), buf_phase ^ 1, abort_flag)) break;
+        if (!tc05::mbar_wait(tc05::smem_u32(&s.full[stage]), phase, abort_flag)) break;
+        tc05::fence_after_sync();
+        const uint32_t w0 = tc05::smem_u32(&s.tiles[stage][0]);
+        const uint32_t x0 = w0 + kBlock * kBlock;
+#pragma unroll
+        for (int ks = 0; ks < kBlock / 32; ++ks)
+          tc05::umma_f8(tmem_base + buf * NT, tc05::smem_desc_sw128(w0 + ks * 32), tc05::smem_desc_sw128(x0 + ks * 32), idesc, ks > 0);
+        tc05::umma_commit(tc05::smem_u32(&s.empty[stage]));
+        tc05::umma_commit(tc05::smem_u32(&s.tmem_full[buf]));
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+        if (++buf == kNarrowBufs) { buf = 0; buf_phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    float(&factor)[2][NT] = s.factor[warp - 2];
+    const float* sb = p.sb + t.expert * p.sb_expert + t.tn * p.sb_row;
+    constexpr int kPer = (NT + 31) / 32;         // tokens whose scale a lane fetches
+    const float* sa[kPer];
+    float next_a[kPer];
+    float next_b = __ldg(sb + (int64_t)kb_lo * p.sb_k);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int64_t row = t.row0 + i * 32 + lane;
+      const bool in = i * 32 + lane < NT && row < t.row_end;
+      sa[i] = p.sa + (in ? row : t.row0) * p.sa_row;
+      next_a[i] = __ldg(sa[i] + (int64_t)kb_lo * p.sa_k);
+    }
+    uint32_t buf = 0, buf_phase = 0, side = 0;
+    for (int kb = kb_lo; kb < kb_hi; ++kb) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i * 32 + lane < NT) factor[side][i * 32 + lane] = __fmul_rn(next_a[i], next_b);
+      __syncwarp();                              // also: every lane has left the other side, which is written next
+      if (kb + 1 < kb_hi) {
+        next_b = __ldg(sb + (int64_t)(kb + 1) * p.sb_k);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) next_a[i] = __ldg(sa[i] + (int64_t)(kb + 1) * p.sa_k);
+      }
+      if (!warp_wait(tc05::smem_u32(&s.tmem_full[buf]), buf_phase, abort_flag)) break;
+      tc05::fence_after_sync();
+      constexpr int kPart = NT < 64 ? NT : 64;   // columns held at a time
+#pragma unroll
+      for (int c0 = 0; c0 < NT; c0 += kPart) {
+        uint32_t r[kPart];
+        tmem_ld_cols<kPart>(tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * NT + c0, r);
+        if (c0 + kPart == NT) {
+          tc05::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&s.tmem_empty[buf]));
+        }
+#pragma unroll
+        for (int j = 0; j < kPart; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&factor[side][c0 + j]);
+          acc[c0 + j] = __fmaf_rn(__uint_as_float(r[j]), f.x, acc[c0 + j]);
+          acc[c0 + j + 1] = __fmaf_rn(__uint_as_float(r[j + 1]), f.y, acc[c0 + j + 1]);
+          acc[c0 + j + 2] = __fmaf_rn(__uint_as_float(r[j + 2]), f.z, acc[c0 + j + 2]);
+          acc[c0 + j + 3] = __fmaf_rn(__uint_as_float(r[j + 3]), f.w, acc[c0 + j + 3]);
+        }
+      }
+      side ^= 1;
+      if (++buf == kNarrowBufs) { buf = 0; buf_phase ^= 1; }
+    }
+    const int64_t n = n0 + quarter * 32 + lane;
+    if (splits == 1) {
+      if (n < p.n && !*abort_flag) {
+        const float b = bias_at(p, n);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          if (t.row0 + j < t.row_end) store_one(p, t.row0 + j, n, __fadd_rn(acc[j], b));
+      }
+    } else {
+      // every copy and every MMA of this CTA has completed (the last tensor-memory buffer is full): the ring is free
+      float* partial = reinterpret_cast<float*>(&s.tiles[0][0]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) partial[j * kBlock + quarter * 32 + lane] = acc[j];
+    }
+  }
+
+  if (splits > 1) {
+    __syncwarp();
+    tc05::cluster_arrive();
+    tc05::cluster_wait();
+    if (warp >= 2 && !*abort_flag) {
+      const int local = (warp & 3) * 32 + lane;
+      const int64_t n = n0 + local;
+      const uint32_t mine = tc05::smem_u32(&s.tiles[0][0]) + local * 4;
+      const float b = n < p.n ? bias_at(p, n) : 0.f;
+      // column j belongs to CTA j % splits; the partial sums are added in rank order
+      for (int j = (int)rank; j < NT; j += splits) {
+        if (t.row0 + j >= t.row_end) break;
+        float sum = 0.f;
+        for (int q = 0; q < splits; ++q) sum = __fadd_rn(sum, ld_cluster(tc05::map_to_cta(mine + j * kBlock * 4, q)));
+        if (n < p.n) store_one(p, t.row0 + j, n, __fadd_rn(sum, b));
+      }
+    }
+    __syncwarp();
+    tc05::cluster_arrive();                      // nobody leaves while its partial sums are being read
+    tc05::cluster_wait();
+  }
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, 2);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc05::fence_after_sync();
+    tc05::tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+// [rows, k] bytes -> tensor map with boxes of 128 bytes x box_rows rows, 128-byte swizzle
+static int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return AMCT_ERR_CUDA;
+  cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)kBlock, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? AMCT_OK : AMCT_ERR_CUDA;
+}
+
+static int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return n;
+}
+
+template <bool GROUPED>
+static int launch_wide(const void* a, const void* b, int64_t ld_a, int64_t ld_b, int64_t rows_b, Params p, int sms, cudaStream_t st) {
+  CUtensorMap ma, mb;
+  int rc = make_map(&ma, a, p.m, p.k, ld_a, kBlock);
+  if (rc != AMCT_OK) return rc;
+  rc = make_map(&mb, b, rows_b, p.k, ld_b, kWideN);
+  if (rc != AMCT_OK) return rc;
+  const size_t smem = sizeof(WideSmem) + 1024;
+  static OncePerDevice attr_set;
+  if (attr_set.first() &&
+      cudaFuncSetAttribute(gemm_fp8_wide_kernel<GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return AMCT_ERR_CUDA;
+  // row tiles per rasterisation group: as many as keep the group's rows of A near 32 MB, a quarter of L2
+  const int64_t g = (32LL << 20) / (p.k * kBlock);
+  p.group_m = (int)(g < 4 ? 4 : g > 64 ? 64 : g);
+  const int64_t tiles_n = (p.n + kWideN - 1) / kWideN;
+  const int64_t row_tiles = (p.m + kBlock - 1) / kBlock + (GROUPED ? (p.experts < p.m ? p.experts : p.m) : 0);
+  const int64_t most = row_tiles * tiles_n;
+  gemm_fp8_wide_kernel<GROUPED><<<(unsigned)(most < sms ? most : sms), kWideThreads, smem, st>>>(ma, mb, p);
+  AMCT_CHECK_LAUNCH();
+  return AMCT_OK;
+}
+
+template <int NT, bool GROUPED>
+static int launch_narrow(const void* a, const void* b, int64_t ld_a, int64_t ld_b, int64_t rows_b, const Params& p, int sms, cudaStream_t st) {
+  CUtensorMap mw, mx;
+  int rc = make_map(&mw, b, rows_b, p.k, ld_b, kBlock);
+  if (rc != AMCT_OK) return rc;
+  rc = make_map(&mx, a, p.m, p.k, ld_a, NT);
+  if (rc != AMCT_OK) return rc;
+  const size_t smem = sizeof(NarrowSmem<NT>) + 1024;
+  static OncePerDevice attr_set;
+  if (attr_set.first() &&
+      cudaFuncSetAttribute(gemm_fp8_narrow_kernel<NT, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return AMCT_ERR_CUDA;
+  const int64_t tiles_n = (p.n + kBlock - 1) / kBlock;
+  // grouped: no more row tiles than this, however the rows are spread over the experts
+  const int64_t row_tiles = GROUPED ? (p.experts < p.m ? p.experts : p.m) + p.m / NT : (p.m + NT - 1) / NT;
+  const int64_t tiles = row_tiles * tiles_n;
+  const int64_t num_kb = (p.k + kBlock - 1) / kBlock;
+  int splits = 1;                                // K split until every SM has its CTAs, four K blocks left for each
+  while (splits < 8 && tiles * splits * 2 <= narrow_ctas<NT>() * sms && num_kb >= splits * 2 * 4) splits *= 2;
+  if (tiles * splits > 0x7fffffffLL) return AMCT_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(tiles * splits), 1, 1);
+  cfg.blockDim = dim3(kNarrowThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, gemm_fp8_narrow_kernel<NT, GROUPED>, mw, mx, p, splits) != cudaSuccess) {
+    cudaGetLastError();
+    return AMCT_ERR_CUDA;
+  }
+  AMCT_CHECK_LAUNCH();
+  return AMCT_OK;
+}
+
+template <bool GROUPED>
+static int launch(const void* a, const void* b, int64_t ld_a, int64_t ld_b, int64_t rows_b, const Params& p, cudaStream_t st) {
+  const int sms = sm_count();
+  if (sms <= 0) return AMCT_ERR_CUDA;
+  // rows that share a weight: all of them, or an expert's on average
+  const int64_t rows = GROUPED ? (p.m + p.experts - 1) / p.experts : p.m;
+  if (rows <= 16) return launch_narrow<16, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
+  if (rows <= 32) return launch_narrow<32, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
+  if (rows <= 64) return launch_narrow<64, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
+  if (rows <= 128) return launch_narrow<128, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
+  return launch_wide<GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
+}
+
+static int check(const void* a, int64_t ld_a, const float* sa, const void* b, int64_t ld_b, const float* sb, int64_t m, int64_t n,
+                 int64_t k, const void* out, int out_kind, int64_t ld_out) {
+  if (m < 0 || n < 0 || k <= 0 || ld_a < k || ld_b < k || ld_out < n) return AMCT_ERR_ARG;
+  if (out_kind < AMCT_GEMM_OUT_F32 || out_kind > AMCT_GEMM_OUT_BF16) return AMCT_ERR_ARG;
+  if (m == 0 || n == 0) return AMCT_OK;
+  if (!a || !b || !sa || !sb || !out) return AMCT_ERR_ARG;
+  if (m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return AMCT_ERR_UNSUPPORTED;     // tensor-map coordinates
+  if (!aligned16(a) || !aligned16(b) || ld_a % 16 != 0 || ld_b % 16 != 0) return AMCT_ERR_ALIGN;
+  const uintptr_t size = out_kind == AMCT_GEMM_OUT_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(out) % size != 0) return AMCT_ERR_ALIGN;
+  return AMCT_OK;
+}
+
+}  // namespace f8g
+}  // namespace amct
+
+extern "C" int amct_gemm_fp8_block(const void* a, const float* a_scale, int64_t a_scale_stride_row, int64_t a_scale_stride_k,
+                                   const void* b, const float* b_scale, int64_t b_scale_stride_row, int64_t b_scale_stride_k,
+                                   int64_t m, int64_t n, int64_t k, int64_t ld_a, int64_t ld_b, const void* bias, int bias_kind,
+                                   void* out, int out_kind, int64_t ld_out, int* status, void* stream) {
+  using namespace amct::f8g;
+  const int rc = check(a, ld_a, a_scale, b, ld_b, b_scale, m, n, k, out, out_kind, ld_out);
+  if (rc != AMCT_OK) return rc;
+  if (bias_kind != AMCT_BIAS_NONE && (bias_kind < AMCT_BIAS_F32 || bias_kind > AMCT_BIAS_BF16 || (n > 0 && !bias))) return AMCT_ERR_ARG;
+  if (m == 0 || n == 0) return AMCT_OK;
+  Params p{};
+  p.m = m; p.n = n; p.k = k;
+  p.sa = a_scale; p.sa_row = a_scale_stride_row; p.sa_k = a_scale_stride_k;
+  p.sb = b_scale; p.sb_row = b_scale_stride_row; p.sb_k = b_scale_stride_k;
+  p.bias = bias; p.bias_kind = bias_kind; p.out = out; p.out_kind = out_kind; p.ld_out = ld_out; p.status = status;
+  return launch<false>(a, b, ld_a, ld_b, n, p, (cudaStream_t)stream);
+}
+
+extern "C" int amct_gemm_fp8_block_grouped(const void* a, const float* a_scale, int64_t a_scale_stride_row, int64_t a_scale_stride_k,
+                                           const int32_t* offsets, int experts, const void* b, const float* b_scale,
+                                           int64_t b_scale_stride_expert, int64_t b_scale_stride_row, int64_t b_scale_stride_k,
+                                           int64_t m, int64_t n, int64_t k, int64_t ld_a, int64_t ld_b, void* out, int out_kind,
+                                           int64_t ld_out, int* status, void* stream) {
+  using namespace amct::f8g;
+  if (experts <= 0) return AMCT_ERR_ARG;
+  const int rc = check(a, ld_a, a_scale, b, ld_b, b_scale, m, n, k, out, out_kind, ld_out);
+  if (rc != AMCT_OK) return rc;
+  if (m == 0 || n == 0) return AMCT_OK;
+  if (!offsets) return AMCT_ERR_ARG;
+  if (experts > kMaxExperts || n > 0x7fffff00LL / experts) return AMCT_ERR_UNSUPPORTED;
+  Params p{};
+  p.m = m; p.n = n; p.k = k;
+  p.sa = a_scale; p.sa_row = a_scale_stride_row; p.sa_k = a_scale_stride_k;
+  p.sb = b_scale; p.sb_expert = b_scale_stride_expert; p.sb_row = b_scale_stride_row; p.sb_k = b_scale_stride_k;
+  p.out = out; p.out_kind = out_kind; p.ld_out = ld_out; p.status = status;
+  p.offsets = offsets; p.experts = experts;
+  return launch<true>(a, b, ld_a, ld_b, (int64_t)experts * n, p, (cudaStream_t)stream);
+}

@@ -341,6 +341,80 @@ int amct_gptq_block(float* w, int64_t n, int64_t ldw, int b, const float* hinv, 
                     const int* offset, int64_t factors_ld, int row_factors, const int* col_group, int bits,
                     float* err, int64_t lde, void* stream);
 
+/* ---- FP8 with a scale for each block of 128: the format of the checkpoints that
+ * amct_pytorch/experimental/quantization/DeepSeekV3.2/deploy.py:48-90 dequantizes, kept as it is ---- */
+enum { AMCT_FP8_BLOCK_TOKEN = 0, AMCT_FP8_BLOCK_TILE = 1 };
+enum { AMCT_FP8_ACT_NONE = 0, AMCT_FP8_ACT_SWIGLU = 1 };
+
+/* E4M3 codes of x and one fp32 scale per block.  AMCT_FP8_BLOCK_TOKEN: 128 columns of one row, scales
+ * [rows, ceil(k / 128)] (activations).  AMCT_FP8_BLOCK_TILE: 128 rows x 128 columns, scales
+ * [ceil(rows / 128), ceil(k / 128)] (weights).  Ragged last blocks hold what is there.
+ *   scale = max|v| / 448 (1 where that is below 2^-126), pow2_scale != 0: the next power of two not below it;
+ *   code  = E4M3(v / scale), round to nearest even, saturating.
+ * v = x, or with AMCT_FP8_ACT_SWIGLU (token blocks only) v[i, c] = silu(x[i, c]) * x[i, k + c] in fp32, x being
+ * [rows, 2 k].  NaN or infinity in a block shows in its scale.  x: fp32 / fp16 / bf16, row stride ld_x; codes uint8,
+ * row stride ld_codes (a multiple of 16 for the GEMMs below); scale (i, b) is written to
+ * scale[i * scale_stride_row + b * scale_stride_k]. */
+int amct_fp8_block_quant(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld_x, int block_kind, int act,
+                         int pow2_scale, void* codes, int64_t ld_codes, float* scale, int64_t scale_stride_row,
+                         int64_t scale_stride_k, void* stream);
+
+/* out[m, n] = sum over 128-wide K blocks kb of a_scale[m, kb] * b_scale[n / 128, kb] * dot(a[m, kb], b[n, kb])
+ * (+ bias[n]): the Linear of such a checkpoint without dequantizing it.  a [m, k] and b [n, k]: E4M3 bytes, K contiguous,
+ * base addresses and leading dimensions multiples of 16 bytes, any k > 0.  a_scale (i, kb) at
+ * a_scale[i * a_scale_stride_row + kb * a_scale_stride_k], b_scale likewise with i = n / 128.  Each K block's dot product is
+ * accumulated on the tensor cores (tcgen05 kind::f8f6f4) and folded into fp32 sums with its scales, then rounded once.
+ * bias_kind: AMCT_BIAS_NONE / F32 / F16 / BF16; out_kind: AMCT_GEMM_OUT_F32 / F16 / BF16.  Results repeat bit for bit.
+ * Bit 1 of *status: a bounded device-side wait expired. */
+int amct_gemm_fp8_block(const void* a, const float* a_scale, int64_t a_scale_stride_row, int64_t a_scale_stride_k,
+                        const void* b, const float* b_scale, int64_t b_scale_stride_row, int64_t b_scale_stride_k,
+                        int64_t m, int64_t n, int64_t k, int64_t ld_a, int64_t ld_b, const void* bias, int bias_kind,
+                        void* out, int out_kind, int64_t ld_out, int* status, void* stream);
+
+/* The same for rows sorted by expert: rows [offsets[e], offsets[e + 1]) of a meet b[e], b [experts, n, k] packed along
+ * experts (expert e begins at row e * n of ld_b bytes).  offsets [experts + 1] int32 on the device, as amct_moe_permute
+ * writes it; values outside [0, m] or descending are clamped.  Rows of out outside every group are left as they were.
+ * experts up to 1024. */
+int amct_gemm_fp8_block_grouped(const void* a, const float* a_scale, int64_t a_scale_stride_row, int64_t a_scale_stride_k,
+                                const int32_t* offsets, int experts, const void* b, const float* b_scale,
+                                int64_t b_scale_stride_expert, int64_t b_scale_stride_row, int64_t b_scale_stride_k,
+                                int64_t m, int64_t n, int64_t k, int64_t ld_a, int64_t ld_b, void* out, int out_kind,
+                                int64_t ld_out, int* status, void* stream);
+
+/* ---- Routed experts: tokens sorted by expert and back
+ * (amct_pytorch/experimental/quantization/DeepSeekV3.2/cores/models/deepseek_v3_2/modeling_deepseek_v3_2.py:522-611) ---- */
+
+/* expert_ids [tokens, topk] contiguous, int32 or int64; a number outside [0, experts) is an assignment that another
+ * rank holds.  The others are sorted stably by expert: row_map [tokens, topk] receives the row of every assignment (-1:
+ * none), offsets [experts + 1] the first row of every expert and, last, the number of rows in use.
+ *   rows[row_map[t, j]] = x[t],  row_scales[row_map[t, j]] = scales[t];  rows from offsets[experts] on are zero.
+ * x [tokens, hidden] (ld_x), rows [tokens * topk, hidden] (ld_rows): elements of elem_bytes = 1, 2 or 4 bytes, copied as
+ * they are.  scales [tokens, scale_cols] fp32 with any strides, or scale_cols = 0.  The same expert may appear more than
+ * once for a token.  workspace: amct_moe_permute_workspace_bytes(tokens * topk, experts) bytes (may be NULL when that is 0),
+ * 4-byte aligned, written before it is read.  experts and topk up to 1024, tokens * topk < 2^31. */
+int64_t amct_moe_permute_workspace_bytes(int64_t assignments, int experts);
+int amct_moe_permute(const void* x, int elem_bytes, int64_t tokens, int64_t hidden, int64_t ld_x, const void* expert_ids,
+                     int ids_are_int64, int topk, int experts, const float* scales, int64_t scale_cols,
+                     int64_t scale_stride_row, int64_t scale_stride_col, void* rows, int64_t ld_rows, float* row_scales,
+                     int64_t row_scale_stride_row, int64_t row_scale_stride_col, int32_t* row_map, int32_t* offsets,
+                     void* workspace, void* stream);
+
+/* out[t] = sum_j weights[t, j] * rows[row_map[t, j]] over the assignments that have a row: fp32, in the order of j,
+ * rounded once to dtype.  weights [tokens, topk] contiguous in weight_dtype, or NULL: ones, which is the gradient of
+ * amct_moe_permute with respect to x.  row_map entries outside [0, n_rows) are skipped. */
+int amct_moe_unpermute(const void* rows, int dtype, int64_t n_rows, int64_t tokens, int topk, int64_t hidden,
+                       int64_t ld_rows, const int32_t* row_map, const void* weights, int weight_dtype, void* out,
+                       int64_t ld_out, void* stream);
+
+/* Gradients of amct_moe_unpermute for a row_map of amct_moe_permute (no row twice):
+ *   grad_rows[row_map[t, j]] = weights[t, j] * grad_out[t], rows from *used_rows (= offsets + experts) on cleared;
+ *   grad_weights[t, j] = dot(grad_out[t], rows[row_map[t, j]]) in fp32, rounded to weight_dtype, 0 without a row.
+ * grad_rows or grad_weights may be NULL; rows is read for grad_weights only. */
+int amct_moe_unpermute_backward(const void* grad_out, const void* rows, int dtype, int64_t n_rows, int64_t tokens,
+                                int topk, int64_t hidden, int64_t ld_grad, int64_t ld_rows, const int32_t* row_map,
+                                const int32_t* used_rows, const void* weights, int weight_dtype, void* grad_rows,
+                                int64_t ld_grad_rows, void* grad_weights, void* stream);
+
 /* ---- Glue of the sharded deploy workload (no counterpart in the reference) ---- */
 
 /* h = x + residual (rounded to dtype; residual may be NULL: h = x); n = round(h * rstd * gamma) with
