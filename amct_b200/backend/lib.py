@@ -26,7 +26,26 @@ FP8_BLOCK = {'token': 0, 'tile': 1}
 FP8_ACT = {None: 0, 'swiglu': 1}
 DSA_DYNAMIC, DSA_LEARNED_CLIP, DSA_CLIP_RATIO, DSA_STATIC, DSA_STATIC_F32 = range(5)
 
+# Argument types of the newer entry points: with them ctypes takes plain numbers, which costs a third of a call's
+# host time less than wrapping every argument (p pointer, i int, l int64)
+_SIGNATURES = {
+    'amct_fp8_block_quant': 'pillliiiplpllp',
+    'amct_gemm_fp8_block': 'ppllpplllllllpipilpp',
+    'amct_gemm_fp8_block_grouped': 'ppllpippllllllllpilpp',
+    'amct_moe_permute': 'pilllpiiiplllplpllpppp',
+    'amct_moe_unpermute': 'pillillppiplp',
+    'amct_moe_unpermute_backward': 'ppillilllpppiplpp',
+}
+_CTYPES = {'p': ctypes.c_void_p, 'i': ctypes.c_int, 'l': ctypes.c_int64}
 _lib = None
+
+
+def declare(lib):
+    """Sets the argument types of the entry points that are called with plain numbers."""
+    for name, letters in _SIGNATURES.items():
+        getattr(lib, name).argtypes = [_CTYPES[c] for c in letters]
+    lib.amct_moe_permute_workspace_bytes.restype = ctypes.c_int64
+    lib.amct_moe_permute_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int]
 
 
 class BackendError(RuntimeError):
@@ -53,7 +72,7 @@ def load():
         lib.amct_minmax_workspace_bytes.argtypes = [ctypes.c_int64]
         lib.amct_minmax_noalloc_max_k.restype = ctypes.c_int64
         lib.amct_mx_tiled_scale_bytes.restype = ctypes.c_int64
-        lib.amct_moe_permute_workspace_bytes.restype = ctypes.c_int64
+        declare(lib)
         lib.amct_mma_peak_ops_per_cta_step.restype = ctypes.c_int64
         _lib = lib
     return _lib

@@ -27,7 +27,8 @@ def _p(t):
 
 
 def _stream():
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    """Handle of the current device's current stream (asked directly: building a torch.cuda.Stream costs 3 us a call)."""
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _need_cuda(*tensors):
@@ -937,6 +938,14 @@ FP8_BLOCK_SIZE = 128
 _SAME = contextlib.nullcontext()
 
 
+def _addr(t):
+    return t.data_ptr() if t is not None else 0
+
+
+def _raw_stream():
+    return _stream().value or 0
+
+
 def _on(*tensors):
     """Context in which the tensors' one device is current; raises when they lie on several, or on the CPU."""
     _need_cuda(*tensors)
@@ -954,8 +963,7 @@ def _cdiv(a, b):
     return (a + b - 1) // b
 
 
-def _is_codes(t):
-    return t.dtype in (torch.float8_e4m3fn, torch.uint8)
+_CODE_DTYPES = (torch.float8_e4m3fn, torch.uint8)
 
 
 def _rows16(codes):
@@ -991,51 +999,57 @@ def fp8_block_quant(x, block='token', act=None, pow2_scale=False):
     if x.dim() < 1 or (act is not None and x.shape[-1] % 2):
         raise ValueError('swiglu needs an even number of columns: the gate half, then the up half')
     with _on(x):
-        k = x.shape[-1] // (2 if act is not None else 1)
-        if x.numel():
+        width = x.shape[-1]
+        k = width // 2 if act is not None else width
+        if x.dim() == 2 and x.is_contiguous():
+            x2, rows, ld = x, x.shape[0], width
+        elif x.numel():
             x2, rows, _, ld = _rows2d(x)
         else:
-            x2, rows, ld = x, (x.shape[:-1].numel() if x.dim() > 1 else 1), x.shape[-1]
+            x2, rows, ld = x, x.shape[:-1].numel(), width
         ld_codes = _cdiv(k, 16) * 16
-        codes = torch.empty((rows, ld_codes), dtype=torch.float8_e4m3fn, device=x.device)
+        codes = torch.empty_strided((rows, k), (ld_codes, 1), dtype=torch.float8_e4m3fn, device=x.device)
         kb = _cdiv(k, FP8_BLOCK_SIZE)
         if tile:
-            scale = torch.empty((_cdiv(rows, FP8_BLOCK_SIZE), kb), dtype=torch.float32, device=x.device)
             stride_row, stride_k = kb, 1
+            shape = (_cdiv(rows, FP8_BLOCK_SIZE), kb)
         else:
-            scale = torch.empty((kb, rows), dtype=torch.float32, device=x.device).t()
             stride_row, stride_k = 1, rows
+            shape = (rows, kb)
+        scale = torch.empty_strided(shape, (stride_row, stride_k), dtype=torch.float32, device=x.device)
         rc = _l.load().amct_fp8_block_quant(
-            _p(x2), c_int(_dt(x2)), c_int64(rows), c_int64(k), c_int64(ld), c_int(_l.FP8_BLOCK[block]), c_int(_l.FP8_ACT[act]),
-            c_int(1 if pow2_scale else 0), _p(codes), c_int64(ld_codes), _p(scale), c_int64(stride_row), c_int64(stride_k), _stream())
+            _addr(x2), _dt(x2), rows, k, ld, _l.FP8_BLOCK[block], _l.FP8_ACT[act],
+            1 if pow2_scale else 0, _addr(codes), ld_codes, _addr(scale), stride_row, stride_k, _raw_stream())
         _l.check(rc, 'amct_fp8_block_quant')
         COUNTERS['launches'] += 1
-    if ld_codes != k:
-        codes = codes[:, :k]
-    return (codes if x.dim() == 2 else codes.view(*x.shape[:-1], k) if ld_codes == k else codes.unflatten(0, x.shape[:-1]) if x.dim() > 1 else codes[0]), scale
+    if x.dim() != 2:
+        codes = codes[0] if x.dim() == 1 else codes.unflatten(0, x.shape[:-1])
+    return codes, scale
 
 
 def _check_fp8_operands(a, a_scale, b, b_scale):
-    if not _is_codes(a) or not _is_codes(b):
+    if a.dtype not in _CODE_DTYPES or b.dtype not in _CODE_DTYPES:
         raise ValueError('a and b must hold E4M3 codes (float8_e4m3fn or uint8)')
     if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
         raise ValueError('the scales must be float32')
-    kb = _cdiv(a.shape[1], FP8_BLOCK_SIZE)
-    if b.shape[-1] != a.shape[1]:
-        raise ValueError(f'a and b must have the same K: {tuple(a.shape)} and {tuple(b.shape)}')
-    if a.shape[1] == 0:
+    m, k = a.shape
+    shape = b.shape
+    kb = _cdiv(k, FP8_BLOCK_SIZE)
+    if shape[-1] != k:
+        raise ValueError(f'a and b must have the same K: {tuple(a.shape)} and {tuple(shape)}')
+    if k == 0:
         raise ValueError('K must not be zero')
-    if tuple(a_scale.shape) != (a.shape[0], kb):
-        raise ValueError(f'a_scale must be [{a.shape[0]}, {kb}], one value for each row and 128 columns')
-    if tuple(b_scale.shape) != (*b.shape[:-2], _cdiv(b.shape[-2], FP8_BLOCK_SIZE), kb):
-        raise ValueError(f'b_scale must have one value for each 128 x 128 tile of b {tuple(b.shape)}')
+    if a_scale.shape != (m, kb):
+        raise ValueError(f'a_scale must be [{m}, {kb}], one value for each row and 128 columns')
+    if b_scale.shape != (*shape[:-2], _cdiv(shape[-2], FP8_BLOCK_SIZE), kb):
+        raise ValueError(f'b_scale must have one value for each 128 x 128 tile of b {tuple(shape)}')
 
 
 def _fp8_out(out, out_dtype, m, n, device):
     if out is None:
         if out_dtype not in _DT:
             raise ValueError('out_dtype must be float32, float16 or bfloat16')
-        return torch.empty((m, n), dtype=out_dtype, device=device)
+        return torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=device)
     if out.dtype not in _DT or tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
         raise ValueError(f'out must be float32 / float16 / bfloat16 [{m}, {n}] with unit inner stride')
     return out
@@ -1064,9 +1078,9 @@ def gemm_fp8_block(a, a_scale, b_nk, b_scale, bias=None, out_dtype=torch.bfloat1
         b_nk, ld_b = _rows16(b_nk)
         prof = _prof_begin()
         rc = _l.load().amct_gemm_fp8_block(
-            _p(a), _p(a_scale), c_int64(a_scale.stride(0)), c_int64(a_scale.stride(1)), _p(b_nk), _p(b_scale),
-            c_int64(b_scale.stride(0)), c_int64(b_scale.stride(1)), c_int64(m), c_int64(n), c_int64(k), c_int64(ld_a), c_int64(ld_b),
-            _p(bias), c_int(bk), _p(out), c_int(_OUT_KIND[out.dtype]), c_int64(out.stride(0) if m > 1 else n), _p(status), _stream())
+            _addr(a), _addr(a_scale), a_scale.stride(0), a_scale.stride(1), _addr(b_nk), _addr(b_scale),
+            b_scale.stride(0), b_scale.stride(1), m, n, k, ld_a, ld_b,
+            _addr(bias), bk, _addr(out), _OUT_KIND[out.dtype], out.stride(0) if m > 1 else n, _addr(status), _raw_stream())
         _l.check(rc, 'amct_gemm_fp8_block')
         COUNTERS['launches'] += 1
         _prof_end(prof, 2 * m * n * k)
@@ -1097,10 +1111,10 @@ def gemm_fp8_block_grouped(a, a_scale, offsets, b_enk, b_scale, out_dtype=torch.
         b_enk, ld_b = _rows16(b_enk)
         prof = _prof_begin()
         rc = _l.load().amct_gemm_fp8_block_grouped(
-            _p(a), _p(a_scale), c_int64(a_scale.stride(0)), c_int64(a_scale.stride(1)), _p(offsets), c_int(experts),
-            _p(b_enk), _p(b_scale), c_int64(b_scale.stride(0)), c_int64(b_scale.stride(1)), c_int64(b_scale.stride(2)),
-            c_int64(m), c_int64(n), c_int64(k), c_int64(ld_a), c_int64(ld_b), _p(out), c_int(_OUT_KIND[out.dtype]),
-            c_int64(out.stride(0) if m > 1 else n), _p(status), _stream())
+            _addr(a), _addr(a_scale), a_scale.stride(0), a_scale.stride(1), _addr(offsets), experts,
+            _addr(b_enk), _addr(b_scale), b_scale.stride(0), b_scale.stride(1), b_scale.stride(2),
+            m, n, k, ld_a, ld_b, _addr(out), _OUT_KIND[out.dtype],
+            out.stride(0) if m > 1 else n, _addr(status), _raw_stream())
         _l.check(rc, 'amct_gemm_fp8_block_grouped')
         COUNTERS['launches'] += 1
         _prof_end(prof, 2 * m * n * k)
@@ -1144,26 +1158,26 @@ def moe_permute(x, expert_ids, num_experts, scales=None):
         x, ld_x = _strided_rows(x)
         expert_ids = expert_ids.contiguous()
         ld_rows = _cdiv(hidden, 16) * 16 if x.element_size() == 1 else hidden
-        rows = torch.empty((n, ld_rows), dtype=x.dtype, device=dev)
-        row_map = torch.empty((tokens, topk), dtype=torch.int32, device=dev)
-        offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+        rows = torch.empty_strided((n, hidden), (ld_rows, 1), dtype=x.dtype, device=dev)
+        row_map = torch.empty_strided((tokens, topk), (topk, 1), dtype=torch.int32, device=dev)
+        offsets = torch.empty_strided((max(num_experts, 0) + 1,), (1,), dtype=torch.int32, device=dev)
         row_scales = None
         cols = 0
         if scales is not None:
             cols = scales.shape[1]
-            row_scales = torch.empty((cols, n), dtype=torch.float32, device=dev).t()
+            row_scales = torch.empty_strided((n, cols), (1, n), dtype=torch.float32, device=dev)
         L = _l.load()
         ws = None
         if n > MOE_FEW_ASSIGNMENTS:
-            ws = torch.empty(max(4, L.amct_moe_permute_workspace_bytes(c_int64(n), c_int(num_experts))), dtype=torch.uint8, device=dev)
+            ws = torch.empty(max(4, L.amct_moe_permute_workspace_bytes(n, num_experts)), dtype=torch.uint8, device=dev)
         rc = L.amct_moe_permute(
-            _p(x), c_int(x.element_size()), c_int64(tokens), c_int64(hidden), c_int64(ld_x), _p(expert_ids),
-            c_int(1 if expert_ids.dtype == torch.int64 else 0), c_int(topk), c_int(num_experts), _p(scales), c_int64(cols),
-            c_int64(scales.stride(0) if cols else 0), c_int64(scales.stride(1) if cols else 0), _p(rows), c_int64(ld_rows),
-            _p(row_scales), c_int64(1), c_int64(n), _p(row_map), _p(offsets), _p(ws), _stream())
+            _addr(x), x.element_size(), tokens, hidden, ld_x, _addr(expert_ids),
+            1 if expert_ids.dtype == torch.int64 else 0, topk, num_experts, _addr(scales), cols,
+            scales.stride(0) if cols else 0, scales.stride(1) if cols else 0, _addr(rows), ld_rows,
+            _addr(row_scales), 1, n, _addr(row_map), _addr(offsets), _addr(ws), _raw_stream())
         _l.check(rc, 'amct_moe_permute')
         COUNTERS['launches'] += 1 if n <= MOE_FEW_ASSIGNMENTS else 3
-    return rows if ld_rows == hidden else rows[:, :hidden], row_scales, MoePlan(row_map, offsets)
+    return rows, row_scales, MoePlan(row_map, offsets)
 
 
 def _check_moe_plan(rows, plan, weights):
@@ -1182,15 +1196,15 @@ def moe_unpermute(rows, plan, weights=None):
     tokens, topk = plan.row_map.shape
     hidden = rows.shape[1]
     with _on(rows, plan.row_map, weights):
-        out = torch.empty((tokens, hidden), dtype=rows.dtype, device=rows.device)
-        if out.numel() == 0:
+        out = torch.empty_strided((tokens, hidden), (hidden, 1), dtype=rows.dtype, device=rows.device)
+        if tokens == 0 or hidden == 0:
             return out
         rows, ld = _strided_rows(rows)
         row_map = plan.row_map.contiguous()
         weights = None if weights is None else weights.contiguous()
         rc = _l.load().amct_moe_unpermute(
-            _p(rows), c_int(_dt(rows)), c_int64(rows.shape[0]), c_int64(tokens), c_int(topk), c_int64(hidden), c_int64(ld),
-            _p(row_map), _p(weights), c_int(0 if weights is None else _dt(weights)), _p(out), c_int64(hidden), _stream())
+            _addr(rows), _dt(rows), rows.shape[0], tokens, topk, hidden, ld,
+            _addr(row_map), _addr(weights), 0 if weights is None else _dt(weights), _addr(out), hidden, _raw_stream())
         _l.check(rc, 'amct_moe_unpermute')
         COUNTERS['launches'] += 1
     return out
@@ -1217,9 +1231,9 @@ def moe_unpermute_backward(grad_out, rows, plan, weights=None, want_rows=True, w
         weights = None if weights is None else weights.contiguous()
         used = plan.offsets[-1:]
         rc = _l.load().amct_moe_unpermute_backward(
-            _p(grad_out), _p(rows), c_int(_dt(rows)), c_int64(rows.shape[0]), c_int64(tokens), c_int(topk), c_int64(hidden),
-            c_int64(ld_g), c_int64(ld), _p(row_map), _p(used), _p(weights), c_int(0 if weights is None else _dt(weights)),
-            _p(grad_rows), c_int64(hidden), _p(grad_weights), _stream())
+            _addr(grad_out), _addr(rows), _dt(rows), rows.shape[0], tokens, topk, hidden,
+            ld_g, ld, _addr(row_map), _addr(used), _addr(weights), 0 if weights is None else _dt(weights),
+            _addr(grad_rows), hidden, _addr(grad_weights), _raw_stream())
         _l.check(rc, 'amct_moe_unpermute_backward')
         COUNTERS['launches'] += 1
     return grad_rows, grad_weights

@@ -7,8 +7,8 @@
 //   code = E4M3(v / s)                     (correctly rounded quotient, then round to nearest even, saturating)
 //
 // v is the input, or silu(gate) * up of the row's two halves.  That product stays in fp32: it is rounded once, to
-// its code.  silu uses the fast exponential and reciprocal (a few 2^-24 relative for gates of ordinary size, far
-// inside the half step of 2^-4 that a code is rounded by).  An infinity makes the block's scale infinite, a NaN makes
+// its code.  silu uses the approximate base-2 exponential and reciprocal (together a few 2^-23 relative for gates of
+// ordinary size, far inside the half step of 2^-4 that a code is rounded by; 0 for gates below -87, where |silu| < 1e-35).  An infinity makes the block's scale infinite, a NaN makes
 // it NaN; both show in whatever the block is multiplied into.
 //
 // Tokens: 16 lanes own one block, 8 elements each; a half warp takes the same block of kRows consecutive rows, so that
@@ -24,44 +24,79 @@ namespace f8b {
 constexpr int kBlock = 128, kThreads = 256;
 constexpr float kMax = 448.f;
 
-// eight consecutive elements of a row as fp32; elements at and behind `left` are zero
+// eight consecutive elements as they are stored, zero at and behind `left`
+template <typename T> struct alignas(16) Raw8 { T v[8]; };
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* src, int left, float (&v)[8]) {
-  constexpr int EV = ElemTraits<T>::kPerVec;
+__device__ __forceinline__ Raw8<T> load8(const T* src, int left) {
+  Raw8<T> r;
   if constexpr (VEC) {
-    if (left >= 8) {
+    constexpr int NV = 8 * (int)sizeof(T) / 16;
 #pragma unroll
-      for (int i = 0; i < 8 / EV; ++i) {
-        const Vec16<T> raw = ld_vec_stream(src + i * EV);
-#pragma unroll
-        for (int e = 0; e < EV; ++e) v[i * EV + e] = ElemTraits<T>::to_f(raw.v[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    }
+    for (int i = 0; i < NV; ++i)
+      reinterpret_cast<uint4*>(&r)[i] = left >= 8 ? __ldcs(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < left ? ElemTraits<T>::to_f(src[e]) : 0.f;
+    for (int e = 0; e < 8; ++e) r.v[e] = e < left ? src[e] : ElemTraits<T>::from_f(0.f);
   }
+  return r;
 }
 
-__device__ __forceinline__ float silu_mul(float g, float u) {
-  return __fmul_rn(__fdividef(g, __fadd_rn(1.f, __expf(-g))), u);
-}
-
-// |v| as an unsigned number: ordered like the magnitudes, a NaN above everything
-__device__ __forceinline__ uint32_t abs_bits8(const float (&v)[8]) {
-  uint32_t m = 0;
+// max|v| with NaN above everything; packed on the 16-bit types
+__device__ __forceinline__ float absmax8(const Raw8<float>& r, float m) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+  for (int e = 0; e < 8; ++e) m = fmax_nan(m, fabsf(r.v[e]));
   return m;
 }
+__device__ __forceinline__ float absmax8(const Raw8<__nv_bfloat16>& r, float m) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+  const __nv_bfloat162 t = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+  return fmax_nan(m, fmax_nan(__low2float(t), __high2float(t)));
+}
+__device__ __forceinline__ float absmax8(const Raw8<__half>& r, float m) {
+  const __half2* h = reinterpret_cast<const __half2*>(&r);
+  const __half2 t = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+  return fmax_nan(m, fmax_nan(__low2float(t), __high2float(t)));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+#ifdef AMCT_CUDA_EMU
+  return exp2f(x);
+#else
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+#endif
+}
+__device__ __forceinline__ float recip_fast(float x) {
+#ifdef AMCT_CUDA_EMU
+  return 1.f / x;
+#else
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+#endif
+}
+// g / (1 + exp(-g)) * u
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  const float e = exp2_fast(__fmul_rn(g, -1.44269504f));
+  return __fmul_rn(__fmul_rn(g, recip_fast(__fadd_rn(1.f, e))), u);
+}
+
+// |v| as unsigned bits: ordered like the magnitudes, a NaN above everything
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 struct Scale {
   float s, recip;
-  bool plain;            // div_by_recip gives the correctly rounded quotient: no step of it leaves the normal range
+  bool plain;            // no step of quotient() leaves the normal range
 };
+// v / s from y = rn(1 / s): one corrected product.  The value in front of the last rounding is within 2^-45 of the
+// quotient, so the result is the correctly rounded one unless the quotient lies that close to the middle of two fp32
+// numbers; a quotient that is exactly between two codes comes out exact.  Two FMAs less than div_by_recip: these kernels
+// are bound by instructions before they are bound by memory.
+__device__ __forceinline__ float quotient(float v, float s, float y) {
+  const float q = __fmul_rn(v, y);
+  return __fmaf_rn(__fmaf_rn(-s, q, v), y, q);
+}
 __device__ __forceinline__ Scale block_scale(uint32_t amax_bits, bool pow2) {
   Scale r;
   r.s = __fdiv_rn(__uint_as_float(amax_bits), kMax);
@@ -79,7 +114,7 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], const Scale& sc) {
   float q[8];
   if (sc.plain) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = div_by_recip(v[e], sc.s, sc.recip);
+    for (int e = 0; e < 8; ++e) q[e] = quotient(v[e], sc.s, sc.recip);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) q[e] = __fdiv_rn(v[e], sc.s);
@@ -116,7 +151,7 @@ struct Params {
 };
 
 template <typename T, bool VEC, int kRows, bool SWIGLU>
-__global__ void __launch_bounds__(kThreads) fp8_token_kernel(Params p, uint32_t kblocks, uint32_t units) {
+__global__ void __launch_bounds__(kThreads, kRows == 4 ? (sizeof(T) == 4 && SWIGLU ? 2 : 4) : 8) fp8_token_kernel(Params p, uint32_t kblocks, uint32_t units) {
   const int lane = threadIdx.x & 15;
   const uint32_t unit = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
   const bool live = unit < units;
@@ -126,34 +161,70 @@ __global__ void __launch_bounds__(kThreads) fp8_token_kernel(Params p, uint32_t 
   const int64_t left64 = p.k - col;
   const int left = !live || left64 <= 0 ? 0 : left64 < 8 ? (int)left64 : 8;
   const T* x = reinterpret_cast<const T*>(p.x) + row0 * p.ld_x + col;
-  float v[kRows][8];
+  Raw8<T> raw[kRows], up[SWIGLU ? kRows : 1];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const bool in = row0 + r < p.rows;
-    load8<T, VEC>(x + r * p.ld_x, in ? left : 0, v[r]);
-    if constexpr (SWIGLU) {
-      float u[8];
-      load8<T, VEC>(x + r * p.ld_x + p.k, in ? left : 0, u);
+    const int have = row0 + r < p.rows ? left : 0;
+    raw[r] = load8<T, VEC>(x + r * p.ld_x, have);
+    if constexpr (SWIGLU) up[r] = load8<T, VEC>(x + r * p.ld_x + p.k, have);
+  }
+  float v[SWIGLU ? kRows : 1][8];
+  uint32_t m[kRows];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[r][e] = silu_mul(v[r][e], u[e]);
+  for (int r = 0; r < kRows; ++r) {
+    if constexpr (SWIGLU) {
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[r][e] = silu_mul(ElemTraits<T>::to_f(raw[r].v[e]), ElemTraits<T>::to_f(up[r].v[e]));
+        top = fmax_nan(top, fabsf(v[r][e]));
+      }
+      m[r] = abs_bits(top);
+    } else {
+      m[r] = abs_bits(absmax8(raw[r], 0.f));
     }
   }
-  float mine = 0.f;
+  // Each lane ends with one row's maximum and works out that row's scale, once: with four rows the lanes split them while
+  // they reduce (5 shuffles where four reductions take 16).
+  uint32_t mine;
+  int my_row;
+  if constexpr (kRows == 4) {
+    const bool b8 = lane & 8, b4 = lane & 4;
+    const uint32_t k0 = max(b8 ? m[2] : m[0], __shfl_xor_sync(0xffffffffu, b8 ? m[0] : m[2], 8));
+    const uint32_t k1 = max(b8 ? m[3] : m[1], __shfl_xor_sync(0xffffffffu, b8 ? m[1] : m[3], 8));
+    mine = max(b4 ? k1 : k0, __shfl_xor_sync(0xffffffffu, b4 ? k0 : k1, 4));
+    my_row = lane >> 2;
+  } else {
+    static_assert(kRows == 1, "one or four rows");
+    mine = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 8));
+    mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 4));
+    my_row = 0;
+  }
+  mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+  mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+  const Scale own = block_scale(mine, p.pow2 != 0);
+  if (live && (lane & (kRows == 4 ? 3 : 15)) == 0 && row0 + my_row < p.rows)
+    p.scale[(row0 + my_row) * p.s_row + (int64_t)kb * p.s_k] = own.s;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    uint32_t m = abs_bits8(v[r]);
+    Scale sc = own;
+    if constexpr (kRows == 4) {
+      const int from = (threadIdx.x & 16) | (r << 2);
+      sc.s = __shfl_sync(0xffffffffu, own.s, from);
+      sc.recip = __shfl_sync(0xffffffffu, own.recip, from);
+      sc.plain = sc.recip != 0.f;
+    }
+    if constexpr (!SWIGLU) {
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const Scale sc = block_scale(m, p.pow2 != 0);
-    if (row0 + r < p.rows) store8<VEC>(p.codes + (row0 + r) * p.ld_codes + col, left, codes8(v[r], sc));
-    if (lane == r) mine = sc.s;
+      for (int e = 0; e < 8; ++e) v[0][e] = ElemTraits<T>::to_f(raw[r].v[e]);
+    }
+    if (row0 + r < p.rows) store8<VEC>(p.codes + (row0 + r) * p.ld_codes + col, left, codes8(v[SWIGLU ? r : 0], sc));
   }
-  if (live && lane < kRows && row0 + lane < p.rows) p.scale[(row0 + lane) * p.s_row + (int64_t)kb * p.s_k] = mine;
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) fp8_tile_kernel(Params p, uint32_t kblocks) {
-  constexpr int kPasses = kBlock / (kThreads / 16);        // 8 rows per thread
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) fp8_tile_kernel(Params p, uint32_t kblocks) {
+  constexpr int kPasses = kBlock / (kThreads / 16);        // 8 rows per thread, held as they were read
   __shared__ uint32_t part[kThreads / 32];
   const uint32_t nb = blockIdx.x / kblocks, kb = blockIdx.x - nb * kblocks;
   const int lane = threadIdx.x & 15, r0 = threadIdx.x >> 4;
@@ -161,15 +232,16 @@ __global__ void __launch_bounds__(kThreads) fp8_tile_kernel(Params p, uint32_t k
   const int64_t left64 = p.k - col;
   const int left = left64 <= 0 ? 0 : left64 < 8 ? (int)left64 : 8;
   const T* x = reinterpret_cast<const T*>(p.x) + row0 * p.ld_x + col;
-  float v[kPasses][8];
-  uint32_t m = 0;
+  Raw8<T> raw[kPasses];
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = r0 + i * (kThreads / 16);
-    load8<T, VEC>(x + r * p.ld_x, row0 + r < p.rows ? left : 0, v[i]);
+    raw[i] = load8<T, VEC>(x + r * p.ld_x, row0 + r < p.rows ? left : 0);
   }
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) m = max(m, abs_bits8(v[i]));
+  for (int i = 0; i < kPasses; ++i) top = absmax8(raw[i], top);
+  uint32_t m = abs_bits(top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
@@ -181,7 +253,10 @@ __global__ void __launch_bounds__(kThreads) fp8_tile_kernel(Params p, uint32_t k
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = r0 + i * (kThreads / 16);
-    if (row0 + r < p.rows) store8<VEC>(p.codes + (row0 + r) * p.ld_codes + col, left, codes8(v[i], sc));
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = ElemTraits<T>::to_f(raw[i].v[e]);
+    if (row0 + r < p.rows) store8<VEC>(p.codes + (row0 + r) * p.ld_codes + col, left, codes8(v, sc));
   }
   if (threadIdx.x == 0) p.scale[(int64_t)nb * p.s_row + (int64_t)kb * p.s_k] = sc.s;
 }

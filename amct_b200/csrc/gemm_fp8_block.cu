@@ -153,7 +153,11 @@ __device__ __forceinline__ float bias_at(const Params& p, int64_t n) {
 }
 
 // ---------------------------------------------------------------------------------------------- wide kernel
-constexpr int kWideN = 256, kWideStages = 4, kWideEpiWarps = 8, kWideThreads = 64 + 32 * kWideEpiWarps;
+// Three warpgroups: TMA and MMA warps in the first (two of its warps idle), eight folding warps in the others.  The launch
+// gives every thread 168 registers; the first group hands back all but 40, the folding groups take 232: 128 sums, two
+// 32-column loads in flight, no spills (40 + 2 x 232 = 3 x 168).
+constexpr int kWideN = 256, kWideStages = 4, kWideEpiWarps = 8, kWideThreads = 128 + 32 * kWideEpiWarps;
+constexpr int kWideRegsFirst = 40, kWideRegsFold = 232;
 constexpr int kWideA = kBlock * kBlock, kWideB = kWideN * kBlock, kWideStageBytes = kWideA + kWideB;
 
 struct __align__(1024) WideSmem {
@@ -165,7 +169,7 @@ struct __align__(1024) WideSmem {
 };
 
 // 128 columns of one row
-__device__ __forceinline__ void store_row128(const Params& p, int64_t row, int64_t n0, float (&acc)[128]) {
+__device__ __forceinline__ void store_row128(const Params& p, int64_t row, int64_t n0, const float (&acc)[128]) {
   const int64_t off = row * p.ld_out + n0;
 #pragma unroll
   for (int c0 = 0; c0 < 128; c0 += 32) {
@@ -232,51 +236,55 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   volatile int* abort_flag = &s.abort_flag;
   const int64_t num_tiles = GROUPED ? (int64_t)s.groups.first[p.experts] * tiles_n : tiles_m * tiles_n;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (tc05::elect_one()) {
-      uint32_t stage = 0, phase = 0;
-      bool alive = true;
-      for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
-        const Tile t = GROUPED ? group_tile<kBlock>(p, s.groups, tile, tiles_n) : dense_tile<kBlock>(p, tile, tiles_m, tiles_n);
-        const int row_b = (int)(t.expert * p.n + t.tn * kWideN);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!tc05::mbar_wait(tc05::smem_u32(&s.empty[stage]), phase ^ 1, abort_flag)) { alive = false; break; }
-          const uint32_t bar = tc05::smem_u32(&s.full[stage]);
-          tc05::mbar_expect_tx(bar, kWideStageBytes);
-          const uint32_t dst = tc05::smem_u32(&s.tiles[stage][0]);
-          tc05::tma_load_2d(dst, &tma_a, bar, kb * kBlock, (int)t.row0);
-          tc05::tma_load_2d(dst + kWideA, &tma_b, bar, kb * kBlock, row_b);
-          if (++stage == kWideStages) { stage = 0; phase ^= 1; }
+  if (warp < 4) {
+    tc05::regs_dec<kWideRegsFirst>();
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer
+      if (tc05::elect_one()) {
+        uint32_t stage = 0, phase = 0;
+        bool alive = true;
+        for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+          const Tile t = GROUPED ? group_tile<kBlock>(p, s.groups, tile, tiles_n) : dense_tile<kBlock>(p, tile, tiles_m, tiles_n);
+          const int row_b = (int)(t.expert * p.n + t.tn * kWideN);
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (!tc05::mbar_wait(tc05::smem_u32(&s.empty[stage]), phase ^ 1, abort_flag)) { alive = false; break; }
+            const uint32_t bar = tc05::smem_u32(&s.full[stage]);
+            tc05::mbar_expect_tx(bar, kWideStageBytes);
+            const uint32_t dst = tc05::smem_u32(&s.tiles[stage][0]);
+            tc05::tma_load_2d(dst, &tma_a, bar, kb * kBlock, (int)t.row0);
+            tc05::tma_load_2d(dst + kWideA, &tma_b, bar, kb * kBlock, row_b);
+            if (++stage == kWideStages) { stage = 0; phase ^= 1; }
+          }
         }
       }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer: one tensor-memory buffer per K block
-    if (tc05::elect_one()) {
-      constexpr uint32_t idesc = tc05::make_idesc(1, 0, 0, kBlock, kWideN);
-      uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
-      bool alive = true;
-      for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!tc05::mbar_wait(tc05::smem_u32(&s.tmem_empty[buf]), buf_phase ^ 1, abort_flag)) { alive = false; break; }
-          if (!tc05::mbar_wait(tc05::smem_u32(&s.full[stage]), phase, abort_flag)) { alive = false; break; }
-          tc05::fence_after_sync();
-          const uint32_t a0 = tc05::smem_u32(&s.tiles[stage][0]);
-          const uint32_t b0 = a0 + kWideA;
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer: one tensor-memory buffer per K block
+      if (tc05::elect_one()) {
+        constexpr uint32_t idesc = tc05::make_idesc(1, 0, 0, kBlock, kWideN);
+        uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
+        bool alive = true;
+        for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (!tc05::mbar_wait(tc05::smem_u32(&s.tmem_empty[buf]), buf_phase ^ 1, abort_flag)) { alive = false; break; }
+            if (!tc05::mbar_wait(tc05::smem_u32(&s.full[stage]), phase, abort_flag)) { alive = false; break; }
+            tc05::fence_after_sync();
+            const uint32_t a0 = tc05::smem_u32(&s.tiles[stage][0]);
+            const uint32_t b0 = a0 + kWideA;
 #pragma unroll
-          for (int ks = 0; ks < kBlock / 32; ++ks)
-            tc05::umma_f8(tmem_base + buf * kWideN, tc05::smem_desc_sw128(a0 + ks * 32), tc05::smem_desc_sw128(b0 + ks * 32), idesc, ks > 0);
-          tc05::umma_commit(tc05::smem_u32(&s.empty[stage]));
-          tc05::umma_commit(tc05::smem_u32(&s.tmem_full[buf]));
-          if (++stage == kWideStages) { stage = 0; phase ^= 1; }
-          if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+            for (int ks = 0; ks < kBlock / 32; ++ks)
+              tc05::umma_f8(tmem_base + buf * kWideN, tc05::smem_desc_sw128(a0 + ks * 32), tc05::smem_desc_sw128(b0 + ks * 32), idesc, ks > 0);
+            tc05::umma_commit(tc05::smem_u32(&s.empty[stage]));
+            tc05::umma_commit(tc05::smem_u32(&s.tmem_full[buf]));
+            if (++stage == kWideStages) { stage = 0; phase ^= 1; }
+            if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+          }
         }
       }
     }
   } else {
+    tc05::regs_inc<kWideRegsFold>();
     // ------------------------------------------------------------ fold and store: 32 rows x 128 columns per warp
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
     uint32_t buf = 0, buf_phase = 0;
     bool alive = true;
     for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {

@@ -24,7 +24,7 @@ namespace moe {
 
 constexpr int kThreads = 256;
 constexpr int kFewAssignments = 1024;
-constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kRounds = 8;
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kRounds = 2;
 constexpr int kSubChunk = kSortThreads * kRounds;          // assignments ranked at a time
 constexpr int kMaxChunks = 512;
 constexpr int kMaxExperts = 1024, kMaxTopk = 1024;
@@ -172,28 +172,6 @@ struct Copy {
   int topk;
 };
 
-// x[token] into its rows; blockIdx.y takes a slice of the columns
-template <typename U>
-__device__ __forceinline__ void copy_token(const Copy& c, int64_t token, const int* pos, int64_t n) {
-  const U* src = reinterpret_cast<const U*>(c.x + token * c.ld_x_bytes);
-  for (int64_t i = (int64_t)blockIdx.y * kThreads + threadIdx.x; i < c.row_units; i += (int64_t)gridDim.y * kThreads) {
-    const U v = __ldcs(src + i);
-    for (int j = 0; j < c.topk; ++j) {
-      const int r = pos[j];
-      if (r >= 0 && r < n) reinterpret_cast<U*>(c.rows + (int64_t)r * c.ld_rows_bytes)[i] = v;
-    }
-  }
-  if (c.scales && blockIdx.y == gridDim.y - 1) {
-    for (int64_t i = threadIdx.x; i < c.scale_cols; i += kThreads) {
-      const float v = __ldg(c.scales + token * c.s_row + i * c.s_col);
-      for (int j = 0; j < c.topk; ++j) {
-        const int r = pos[j];
-        if (r >= 0 && r < n) c.row_scales[(int64_t)r * c.o_row + i * c.o_col] = v;
-      }
-    }
-  }
-}
-
 template <typename U> __device__ __forceinline__ U zero_unit();
 template <> __device__ __forceinline__ uint4 zero_unit<uint4>() { return make_uint4(0, 0, 0, 0); }
 template <> __device__ __forceinline__ uint2 zero_unit<uint2>() { return make_uint2(0, 0); }
@@ -201,10 +179,33 @@ template <> __device__ __forceinline__ unsigned zero_unit<unsigned>() { return 0
 template <> __device__ __forceinline__ unsigned short zero_unit<unsigned short>() { return 0; }
 template <> __device__ __forceinline__ unsigned char zero_unit<unsigned char>() { return 0; }
 
-// rows used + part, used + part + parts, .. below n cleared
+// x[token] into its rows; blockIdx.y takes a slice of the columns.  pos[j] < 0: row ~pos[j] is cleared instead, where
+// CLEAR says that such entries are rows, else there is nothing to do.
+template <typename U, bool CLEAR>
+__device__ __forceinline__ void copy_token(const Copy& c, int64_t token, const int* pos, int64_t n) {
+  const U* src = reinterpret_cast<const U*>(c.x + token * c.ld_x_bytes);
+  for (int64_t i = (int64_t)blockIdx.y * kThreads + threadIdx.x; i < c.row_units; i += (int64_t)gridDim.y * kThreads) {
+    const U v = __ldcs(src + i);
+    for (int j = 0; j < c.topk; ++j) {
+      const int p = pos[j], r = CLEAR && p < 0 ? ~p : p;
+      if (r >= 0 && r < n) reinterpret_cast<U*>(c.rows + (int64_t)r * c.ld_rows_bytes)[i] = CLEAR && p < 0 ? zero_unit<U>() : v;
+    }
+  }
+  if (c.scales && blockIdx.y == gridDim.y - 1) {
+    for (int64_t i = threadIdx.x; i < c.scale_cols; i += kThreads) {
+      const float v = __ldg(c.scales + token * c.s_row + i * c.s_col);
+      for (int j = 0; j < c.topk; ++j) {
+        const int p = pos[j], r = CLEAR && p < 0 ? ~p : p;
+        if (r >= 0 && r < n) c.row_scales[(int64_t)r * c.o_row + i * c.o_col] = CLEAR && p < 0 ? 0.f : v;
+      }
+    }
+  }
+}
+
+// rows [used, n) cleared, spread over blockIdx.x
 template <typename U>
-__device__ __forceinline__ void clear_rows(const Copy& c, int64_t used, int64_t n, unsigned part, unsigned parts) {
-  for (int64_t r = used + part; r < n; r += parts) {
+__device__ __forceinline__ void clear_rows(const Copy& c, int64_t used, int64_t n) {
+  for (int64_t r = used + blockIdx.x; r < n; r += gridDim.x) {
     U* dst = reinterpret_cast<U*>(c.rows + r * c.ld_rows_bytes);
     for (int64_t i = (int64_t)blockIdx.y * kThreads + threadIdx.x; i < c.row_units; i += (int64_t)gridDim.y * kThreads) dst[i] = zero_unit<U>();
     if (c.scales && blockIdx.y == gridDim.y - 1)
@@ -212,8 +213,8 @@ __device__ __forceinline__ void clear_rows(const Copy& c, int64_t used, int64_t 
   }
 }
 
-// Few assignments: ranking and copy in one launch.  Block t < tokens owns a token; block `tokens` writes the offsets and
-// clears the rows that nobody has.
+// Few assignments: ranking and copy in one launch.  Block t < tokens owns a token; block `tokens` writes the offsets.  An
+// assignment without an expert is ranked behind all others: its place is one of the rows to clear.
 template <typename U>
 __global__ void __launch_bounds__(kThreads) moe_few_kernel(Sort p, Copy c) {
   __shared__ int pos[kFewAssignments];
@@ -227,16 +228,17 @@ __global__ void __launch_bounds__(kThreads) moe_few_kernel(Sort p, Copy c) {
       int ahead = 0;
       for (int i = lane; i < n; i += 32) {
         const int o = expert_at(p.ids, p.wide, i, p.experts);
-        ahead += o >= 0 && (o < e || (o == e && i < me)) ? 1 : 0;
+        // as unsigned numbers -1 is the largest expert
+        ahead += (unsigned)o < (unsigned)e || (o == e && i < me) ? 1 : 0;
       }
       ahead = warp_sum(ahead);
       if (lane == 0) {
-        pos[j] = e >= 0 ? ahead : -1;
-        if (blockIdx.y == 0) p.row_map[me] = pos[j];
+        pos[j] = e >= 0 ? ahead : ~ahead;
+        if (blockIdx.y == 0) p.row_map[me] = e >= 0 ? ahead : -1;
       }
     }
     __syncthreads();
-    copy_token<U>(c, blockIdx.x, pos, n);
+    copy_token<U, true>(c, blockIdx.x, pos, n);
   } else {
     for (int e = threadIdx.x; e < p.experts; e += kThreads) hist[e] = 0;
     __syncthreads();
@@ -248,15 +250,14 @@ __global__ void __launch_bounds__(kThreads) moe_few_kernel(Sort p, Copy c) {
     block_exclusive_scan<kThreads>(hist, p.experts, first, warp_total);
     if (blockIdx.y == 0)
       for (int e = threadIdx.x; e <= p.experts; e += kThreads) p.offsets[e] = first[e];
-    clear_rows<U>(c, first[p.experts], n, 0, 1);
   }
 }
 
 template <typename U>
 __global__ void __launch_bounds__(kThreads) moe_copy_kernel(Copy c, const int* row_map, const int* used, int64_t n) {
-  copy_token<U>(c, blockIdx.x, row_map + (int64_t)blockIdx.x * c.topk, n);
+  copy_token<U, false>(c, blockIdx.x, row_map + (int64_t)blockIdx.x * c.topk, n);
   const int have = __ldg(used);
-  clear_rows<U>(c, have < 0 ? 0 : have, n, blockIdx.x, gridDim.x);
+  clear_rows<U>(c, have < 0 ? 0 : have, n);
 }
 
 // ---------------------------------------------------------------------------------------------- back to tokens
@@ -281,6 +282,28 @@ struct Combine {
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
+// acc += sum over u < U of wt[u] * rows[pos[u]], columns [V i, V i + V).  All U loads are issued before the first is used,
+// without a branch between them: an assignment without a row reads row 0 and is left out by a select.
+template <typename T, int V, int U>
+__device__ __forceinline__ void combine_some(const T* rows, int64_t ld, int64_t i, const int* pos, const float* wt, float (&acc)[V]) {
+  Pack<T, V> y[U];
+  int r[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    r[u] = pos[u];
+    y[u] = *reinterpret_cast<const Pack<T, V>*>(rows + (int64_t)max(r[u], 0) * ld + i * V);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float w = wt[u];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float sum = __fmaf_rn(w, ElemTraits<T>::to_f(y[u].v[e]), acc[e]);
+      acc[e] = r[u] >= 0 ? sum : acc[e];
+    }
+  }
+}
+
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) moe_combine_kernel(Combine p) {
   __shared__ int pos[kMaxTopk];
@@ -300,19 +323,17 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(Combine p) {
     float acc[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.f;
-    for (int j0 = 0; j0 < p.topk; j0 += 8) {
-      Pack<T, V> y[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)                // eight rows' loads in flight
-        if (j0 + u < p.topk && pos[j0 + u] >= 0)
-          y[u] = *reinterpret_cast<const Pack<T, V>*>(rows + (int64_t)pos[j0 + u] * p.ld_rows + i * V);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        if (j0 + u < p.topk && pos[j0 + u] >= 0) {
-          const float w = wt[j0 + u];
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[e] = __fmaf_rn(w, ElemTraits<T>::to_f(y[u].v[e]), acc[e]);
-        }
+    if (p.n_rows > 0) {
+      int j = 0;
+      for (; j + 8 <= p.topk; j += 8) combine_some<T, V, 8>(rows, p.ld_rows, i, pos + j, wt + j, acc);
+      switch (p.topk - j) {                      // what is left in one go too: 4 + 2 rows are 10 % slower than 6
+        case 7: combine_some<T, V, 7>(rows, p.ld_rows, i, pos + j, wt + j, acc); break;
+        case 6: combine_some<T, V, 6>(rows, p.ld_rows, i, pos + j, wt + j, acc); break;
+        case 5: combine_some<T, V, 5>(rows, p.ld_rows, i, pos + j, wt + j, acc); break;
+        case 4: combine_some<T, V, 4>(rows, p.ld_rows, i, pos + j, wt + j, acc); break;
+        case 3: combine_some<T, V, 3>(rows, p.ld_rows, i, pos + j, wt + j, acc); break;
+        case 2: combine_some<T, V, 2>(rows, p.ld_rows, i, pos + j, wt + j, acc); break;
+        case 1: combine_some<T, V, 1>(rows, p.ld_rows, i, pos + j, wt + j, acc); break;
       }
     }
     Pack<T, V> o;
@@ -336,79 +357,93 @@ struct CombineBackward {
   void* grad_weights;          // [tokens, topk] in weight_dtype, or null
 };
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) moe_combine_backward_kernel(CombineBackward p) {
-  constexpr int U = 8;
-  __shared__ int pos[kMaxTopk];
-  __shared__ float wt[kMaxTopk];
-  __shared__ float part[kThreads / 32][U];
+// U assignments of a token, from pos / wt on: their rows' gradients and the dot products for their weights' gradients
+// (part: [kThreads / 32][8] in shared memory).  The whole block takes part.
+template <typename T, int V, int U>
+__device__ __forceinline__ void backward_some(const CombineBackward& p, const T* g_row, int64_t first, const int* pos, const float* wt,
+                                              float (*part)[8]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t token = blockIdx.x;
-  for (int j = threadIdx.x; j < p.topk; j += kThreads) {
-    const int64_t i = token * p.topk + j;
-    const int r = p.row_map[i];
-    pos[j] = r >= 0 && r < p.n_rows ? r : -1;
-    wt[j] = p.weights ? weight_at(p.weights, p.weight_dtype, i) : 1.f;
-  }
-  __syncthreads();
-  const T* g_row = reinterpret_cast<const T*>(p.grad_out) + token * p.ld_grad;
   const T* rows = reinterpret_cast<const T*>(p.rows);
   T* grad_rows = reinterpret_cast<T*>(p.grad_rows);
   const int64_t vecs = p.hidden / V;
-  for (int j0 = 0; j0 < p.topk; j0 += U) {
-    float dot[U];
+  int r[U];
+  float w[U], dot[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) dot[u] = 0.f;
-    for (int64_t i = threadIdx.x; i < vecs; i += kThreads) {
-      const Pack<T, V> g = *reinterpret_cast<const Pack<T, V>*>(g_row + i * V);
-      Pack<T, V> y[U];
-      if (p.grad_weights) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (j0 + u < p.topk && pos[j0 + u] >= 0)
-            y[u] = *reinterpret_cast<const Pack<T, V>*>(rows + (int64_t)pos[j0 + u] * p.ld_rows + i * V);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (j0 + u < p.topk && pos[j0 + u] >= 0) {
-          if (p.grad_weights) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) dot[u] = __fmaf_rn(ElemTraits<T>::to_f(g.v[e]), ElemTraits<T>::to_f(y[u].v[e]), dot[u]);
-          }
-          if (grad_rows) {
-            const float w = wt[j0 + u];
-            Pack<T, V> o;
-#pragma unroll
-            for (int e = 0; e < V; ++e) o.v[e] = ElemTraits<T>::from_f(__fmul_rn(w, ElemTraits<T>::to_f(g.v[e])));
-            *reinterpret_cast<Pack<T, V>*>(grad_rows + (int64_t)pos[j0 + u] * p.ld_grad_rows + i * V) = o;
-          }
-        }
-      }
-    }
+  for (int u = 0; u < U; ++u) {
+    r[u] = pos[u];
+    w[u] = wt[u];
+    dot[u] = 0.f;
+  }
+  for (int64_t i = threadIdx.x; i < vecs; i += kThreads) {
+    const Pack<T, V> g = *reinterpret_cast<const Pack<T, V>*>(g_row + i * V);
     if (p.grad_weights) {
+      Pack<T, V> y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) y[u] = *reinterpret_cast<const Pack<T, V>*>(rows + (int64_t)max(r[u], 0) * p.ld_rows + i * V);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+        for (int e = 0; e < V; ++e) dot[u] = __fmaf_rn(ElemTraits<T>::to_f(g.v[e]), ElemTraits<T>::to_f(y[u].v[e]), dot[u]);
       }
-      if (lane == 0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) part[warp][u] = dot[u];
-      }
-      __syncthreads();
-      if (threadIdx.x < U && j0 + (int)threadIdx.x < p.topk) {
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) sum += part[w][threadIdx.x];
-        const int64_t i = token * p.topk + j0 + threadIdx.x;
-        switch (p.weight_dtype) {
-          case AMCT_DTYPE_F16: reinterpret_cast<__half*>(p.grad_weights)[i] = __float2half_rn(sum); break;
-          case AMCT_DTYPE_BF16: reinterpret_cast<__nv_bfloat16*>(p.grad_weights)[i] = __float2bfloat16_rn(sum); break;
-          default: reinterpret_cast<float*>(p.grad_weights)[i] = sum;
-        }
-      }
-      __syncthreads();
     }
+    if (grad_rows) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        Pack<T, V> o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o.v[e] = ElemTraits<T>::from_f(__fmul_rn(w[u], ElemTraits<T>::to_f(g.v[e])));
+        if (r[u] >= 0) *reinterpret_cast<Pack<T, V>*>(grad_rows + (int64_t)r[u] * p.ld_grad_rows + i * V) = o;
+      }
+    }
+  }
+  if (p.grad_weights) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+      if (lane == 0) part[warp][u] = r[u] >= 0 ? dot[u] : 0.f;      // what was read for an absent row is left out here
+    }
+    __syncthreads();
+    if (threadIdx.x < U) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kThreads / 32; ++k) sum += part[k][threadIdx.x];
+      const int64_t i = first + threadIdx.x;
+      switch (p.weight_dtype) {
+        case AMCT_DTYPE_F16: reinterpret_cast<__half*>(p.grad_weights)[i] = __float2half_rn(sum); break;
+        case AMCT_DTYPE_BF16: reinterpret_cast<__nv_bfloat16*>(p.grad_weights)[i] = __float2bfloat16_rn(sum); break;
+        default: reinterpret_cast<float*>(p.grad_weights)[i] = sum;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) moe_combine_backward_kernel(CombineBackward p) {
+  __shared__ int pos[kMaxTopk];
+  __shared__ float wt[kMaxTopk];
+  __shared__ float part[kThreads / 32][8];
+  const int64_t token = blockIdx.x, first = token * p.topk;
+  for (int j = threadIdx.x; j < p.topk; j += kThreads) {
+    const int r = p.row_map[first + j];
+    pos[j] = r >= 0 && r < p.n_rows ? r : -1;
+    wt[j] = p.weights ? weight_at(p.weights, p.weight_dtype, first + j) : 1.f;
+  }
+  __syncthreads();
+  const T* g_row = reinterpret_cast<const T*>(p.grad_out) + token * p.ld_grad;
+  T* grad_rows = reinterpret_cast<T*>(p.grad_rows);
+  const int64_t vecs = p.hidden / V;
+  int j = 0;
+  for (; j + 8 <= p.topk; j += 8) backward_some<T, V, 8>(p, g_row, first + j, pos + j, wt + j, part);
+  switch (p.topk - j) {
+    case 7: backward_some<T, V, 7>(p, g_row, first + j, pos + j, wt + j, part); break;
+    case 6: backward_some<T, V, 6>(p, g_row, first + j, pos + j, wt + j, part); break;
+    case 5: backward_some<T, V, 5>(p, g_row, first + j, pos + j, wt + j, part); break;
+    case 4: backward_some<T, V, 4>(p, g_row, first + j, pos + j, wt + j, part); break;
+    case 3: backward_some<T, V, 3>(p, g_row, first + j, pos + j, wt + j, part); break;
+    case 2: backward_some<T, V, 2>(p, g_row, first + j, pos + j, wt + j, part); break;
+    case 1: backward_some<T, V, 1>(p, g_row, first + j, pos + j, wt + j, part); break;
   }
   if (grad_rows) {
     const int used = __ldg(p.used);

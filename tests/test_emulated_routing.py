@@ -20,7 +20,11 @@ def library(tmp_path_factory):
                            '-fPIC', '-shared', '-x', 'c++', '-include', os.path.join(E.EMU, 'cuda_emu_routing.h'), '-I', E.CUDA_INCLUDE,
                            os.path.join(E.CSRC, 'fp8_block_quant.cu'), os.path.join(E.CSRC, 'moe_permute.cu'), '-o', out, '-lpthread'])
     handle = ctypes.CDLL(out)
-    handle.amct_moe_permute_workspace_bytes.restype = ctypes.c_int64
+    from amct_b200.backend import lib
+    monkeypatch = pytest.MonkeyPatch()
+    monkeypatch.setattr(lib, '_SIGNATURES', {n: s for n, s in lib._SIGNATURES.items() if hasattr(handle, n)})
+    lib.declare(handle)
+    monkeypatch.undo()
     return handle
 
 
