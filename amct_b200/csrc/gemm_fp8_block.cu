@@ -100,14 +100,15 @@ __device__ __forceinline__ void build_groups(const Params& p, GroupTable& g) {
 }
 
 struct Tile {
-  int64_t row0, row_end;       // rows [row0, min(row0 + tile, row_end)) are this tile's
-  int64_t tn;                  // column tile
+  int row0, row_end;           // rows [row0, min(row0 + tile, row_end)) are this tile's
+  int tn;                      // column tile
   int expert;
 };
 
+// Tile numbers are 32-bit (the launcher sees to it): a 64-bit division per tile would cost every role its registers.
 // Grouped: all tiles of a group lie together, row tiles fastest, so that CTAs running at one time share its weight.
 template <int TILE>
-__device__ __forceinline__ Tile group_tile(const Params& p, const GroupTable& g, int64_t tile, int64_t tiles_n) {
+__device__ __forceinline__ Tile group_tile(const Params& p, const GroupTable& g, uint32_t tile, uint32_t tiles_n) {
   const int want = (int)(tile / tiles_n);
   int lo = 0, hi = p.experts;                    // first[lo] <= want < first[hi]
   while (hi - lo > 1) {
@@ -116,24 +117,24 @@ __device__ __forceinline__ Tile group_tile(const Params& p, const GroupTable& g,
   }
   Tile t;
   t.expert = lo;
-  const int64_t rel = tile - (int64_t)g.first[lo] * tiles_n;
-  const int64_t mt = g.first[lo + 1] - g.first[lo];
-  t.tn = rel / mt;
-  t.row0 = g.bound[lo] + (rel - t.tn * mt) * TILE;
+  const uint32_t rel = tile - (uint32_t)g.first[lo] * tiles_n;
+  const uint32_t mt = (uint32_t)(g.first[lo + 1] - g.first[lo]);
+  t.tn = (int)(rel / mt);
+  t.row0 = g.bound[lo] + (int)(rel - (uint32_t)t.tn * mt) * TILE;
   t.row_end = g.bound[lo + 1];
   return t;
 }
 
 template <int TILE>
-__device__ __forceinline__ Tile dense_tile(const Params& p, int64_t tile, int64_t tiles_m, int64_t tiles_n) {
-  const int64_t per_group = (int64_t)p.group_m * tiles_n;
-  const int64_t g = tile / per_group, r = tile - g * per_group;
-  const int64_t m0 = g * p.group_m;
-  const int64_t gm = (tiles_m - m0) < p.group_m ? (tiles_m - m0) : p.group_m;
+__device__ __forceinline__ Tile dense_tile(const Params& p, uint32_t tile, uint32_t tiles_m, uint32_t tiles_n) {
+  const uint32_t per_group = (uint32_t)p.group_m * tiles_n;
+  const uint32_t g = tile / per_group, r = tile - g * per_group;
+  const uint32_t m0 = g * (uint32_t)p.group_m;
+  const uint32_t gm = tiles_m - m0 < (uint32_t)p.group_m ? tiles_m - m0 : (uint32_t)p.group_m;
   Tile t;
-  t.tn = r / gm;
-  t.row0 = (m0 + (r - t.tn * gm)) * TILE;
-  t.row_end = p.m;
+  t.tn = (int)(r / gm);
+  t.row0 = (int)(m0 + (r - (uint32_t)t.tn * gm)) * TILE;
+  t.row_end = (int)p.m;
   t.expert = 0;
   return t;
 }
@@ -160,17 +161,26 @@ constexpr int kWideN = 256, kWideStages = 4, kWideEpiWarps = 8, kWideThreads = 1
 constexpr int kWideRegsFirst = 40, kWideRegsFold = 232;
 constexpr int kWideA = kBlock * kBlock, kWideB = kWideN * kBlock, kWideStageBytes = kWideA + kWideB;
 
+constexpr int kTurnBytes = 32 * 66;      // per folding warp: 32 rows of 64 bytes, padded to an odd number of 16-bit words
+
 struct __align__(1024) WideSmem {
   uint8_t tiles[kWideStages][kWideStageBytes];
+  uint8_t turn[kWideEpiWarps][kTurnBytes];
   GroupTable groups;
   uint64_t full[kWideStages], empty[kWideStages], tmem_full[2], tmem_empty[2];
   uint32_t tmem_base;
   volatile int abort_flag;
 };
 
-// 128 columns of one row
-__device__ __forceinline__ void store_row128(const Params& p, int64_t row, int64_t n0, const float (&acc)[128]) {
-  const int64_t off = row * p.ld_out + n0;
+
+// A folding warp's 32 rows x 128 columns; `row` is this lane's.  Rows that begin at 16 bytes leave as vectors, a lane its own
+// row.  Others (an odd N) are turned around in shared memory, 64 bytes of every row at a time, and leave 32 consecutive
+// outputs per instruction: 2-byte stores of 32 different rows cost 2.6 x the whole kernel's time (777 x 5001 x 4000).
+__device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int row_end, int lane, int64_t n0, float (&acc)[128], uint8_t* turn) {
+  const int row = warp_row0 + lane;
+  const int esize = p.out_kind == AMCT_GEMM_OUT_F32 ? 4 : 2;
+  uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
+  const bool vectors = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(p.ld_out * esize)) & 15) == 0;
 #pragma unroll
   for (int c0 = 0; c0 < 128; c0 += 32) {
     const int64_t left = p.n - (n0 + c0);
@@ -182,25 +192,40 @@ __device__ __forceinline__ void store_row128(const Params& p, int64_t row, int64
 #pragma unroll
       for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], j < left ? bias_at(p, n0 + c0 + j) : 0.f);
     }
-    if (p.out_kind == AMCT_GEMM_OUT_F32) {
-      float* o = reinterpret_cast<float*>(p.out) + off + c0;
-      if (left >= 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+    uint32_t h[16];
+    if (esize == 2) epi_pack16(y, p.out_kind == AMCT_GEMM_OUT_BF16, h);
+    if (vectors && left >= 32) {
+      if (row < row_end) {
+        uint8_t* o = out + ((int64_t)row * p.ld_out + n0 + c0) * esize;
+        if (esize == 4) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(o + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
-      } else {
+          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(o + 4 * j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) if (j < left) o[j] = y[j];
+          for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(o + 4 * j) = make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
+        }
       }
+      continue;
+    }
+    if (esize == 2) {
+      uint16_t* mine = reinterpret_cast<uint16_t*>(turn) + lane * 33;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) mine[j] = (uint16_t)(h[j >> 1] >> (16 * (j & 1)));
+      __syncwarp();
+      for (int r = 0; r < 32 && warp_row0 + r < row_end; ++r)
+        if (lane < left) reinterpret_cast<uint16_t*>(out)[(int64_t)(warp_row0 + r) * p.ld_out + n0 + c0 + lane] = reinterpret_cast<const uint16_t*>(turn)[r * 33 + lane];
+      __syncwarp();
     } else {
-      uint32_t h[16];
-      epi_pack16(y, p.out_kind == AMCT_GEMM_OUT_BF16, h);
-      uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + off + c0;
-      if (left >= 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(o + 2 * j) = make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
-      } else {
+      for (int part = 0; part < 2; ++part) {     // 16 columns of every row
+        float* mine = reinterpret_cast<float*>(turn) + lane * 16;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) if (j < left) o[j] = (uint16_t)(h[j >> 1] >> (16 * (j & 1)));
+        for (int j = 0; j < 16; ++j) mine[(j + lane) & 15] = y[part * 16 + j];
+        __syncwarp();
+        const int half = lane >> 4, c = lane & 15;
+        for (int r = half; r < 32 && warp_row0 + r < row_end; r += 2)
+          if (part * 16 + c < left) reinterpret_cast<float*>(out)[(int64_t)(warp_row0 + r) * p.ld_out + n0 + c0 + part * 16 + c] = reinterpret_cast<const float*>(turn)[r * 16 + ((c + r) & 15)];
+        __syncwarp();
       }
     }
   }
@@ -213,8 +238,8 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   WideSmem& s = *reinterpret_cast<WideSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_kb = (int)((p.k + kBlock - 1) / kBlock);
-  const int64_t tiles_n = (p.n + kWideN - 1) / kWideN;
-  const int64_t tiles_m = (p.m + kBlock - 1) / kBlock;
+  const uint32_t tiles_n = (uint32_t)((p.n + kWideN - 1) / kWideN);
+  const uint32_t tiles_m = (uint32_t)((p.m + kBlock - 1) / kBlock);
 
   if (threadIdx.x == 0) {
     s.abort_flag = 0;
@@ -234,7 +259,7 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   tc05::fence_after_sync();
   const uint32_t tmem_base = s.tmem_base;
   volatile int* abort_flag = &s.abort_flag;
-  const int64_t num_tiles = GROUPED ? (int64_t)s.groups.first[p.experts] * tiles_n : tiles_m * tiles_n;
+  const uint32_t num_tiles = (GROUPED ? (uint32_t)s.groups.first[p.experts] : tiles_m) * tiles_n;
 
   if (warp < 4) {
     tc05::regs_dec<kWideRegsFirst>();
@@ -243,15 +268,15 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       if (tc05::elect_one()) {
         uint32_t stage = 0, phase = 0;
         bool alive = true;
-        for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+        for (uint32_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
           const Tile t = GROUPED ? group_tile<kBlock>(p, s.groups, tile, tiles_n) : dense_tile<kBlock>(p, tile, tiles_m, tiles_n);
-          const int row_b = (int)(t.expert * p.n + t.tn * kWideN);
+          const int row_b = t.expert * (int)p.n + t.tn * kWideN;
           for (int kb = 0; kb < num_kb; ++kb) {
             if (!tc05::mbar_wait(tc05::smem_u32(&s.empty[stage]), phase ^ 1, abort_flag)) { alive = false; break; }
             const uint32_t bar = tc05::smem_u32(&s.full[stage]);
             tc05::mbar_expect_tx(bar, kWideStageBytes);
             const uint32_t dst = tc05::smem_u32(&s.tiles[stage][0]);
-            tc05::tma_load_2d(dst, &tma_a, bar, kb * kBlock, (int)t.row0);
+            tc05::tma_load_2d(dst, &tma_a, bar, kb * kBlock, t.row0);
             tc05::tma_load_2d(dst + kWideA, &tma_b, bar, kb * kBlock, row_b);
             if (++stage == kWideStages) { stage = 0; phase ^= 1; }
           }
@@ -263,7 +288,7 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         constexpr uint32_t idesc = tc05::make_idesc(1, 0, 0, kBlock, kWideN);
         uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
         bool alive = true;
-        for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+        for (uint32_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
           for (int kb = 0; kb < num_kb; ++kb) {
             if (!tc05::mbar_wait(tc05::smem_u32(&s.tmem_empty[buf]), buf_phase ^ 1, abort_flag)) { alive = false; break; }
             if (!tc05::mbar_wait(tc05::smem_u32(&s.full[stage]), phase, abort_flag)) { alive = false; break; }
@@ -287,13 +312,13 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     uint32_t buf = 0, buf_phase = 0;
     bool alive = true;
-    for (int64_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+    for (uint32_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
       const Tile t = GROUPED ? group_tile<kBlock>(p, s.groups, tile, tiles_n) : dense_tile<kBlock>(p, tile, tiles_m, tiles_n);
-      const int64_t row = t.row0 + quarter * 32 + lane;
-      const int64_t n0 = t.tn * kWideN + half * 128;
+      const int row = t.row0 + quarter * 32 + lane;
+      const int64_t n0 = (int64_t)t.tn * kWideN + half * 128;
       const bool row_in = row < t.row_end, cols_in = n0 < p.n;
-      const float* sa = p.sa + (row_in ? row : t.row0) * p.sa_row;
-      const float* sb = p.sb + t.expert * p.sb_expert + (cols_in ? n0 / kBlock : 0) * p.sb_row;
+      const float* sa = p.sa + (int64_t)(row_in ? row : t.row0) * p.sa_row;
+      const float* sb = p.sb + (int64_t)t.expert * p.sb_expert + (cols_in ? n0 / kBlock : 0) * p.sb_row;
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
@@ -323,7 +348,7 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         }
         if (++buf == 2) { buf = 0; buf_phase ^= 1; }
       }
-      if (alive && row_in && cols_in) store_row128(p, row, n0, acc);
+      if (alive && cols_in) store_rows(p, t.row0 + quarter * 32, t.row_end, lane, n0, acc, s.turn[warp - 4]);
       __syncwarp();
     }
   }
@@ -341,28 +366,30 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
 }
 
 // ---------------------------------------------------------------------------------------------- narrow kernel
-constexpr int kNarrowThreads = 192;
-constexpr int kNarrowBufs = 4;
+constexpr int kNarrowBufs = 4, kMaxSplits = 8;
 
-// Up to 64 tokens two CTAs share an SM (about 110 KB of shared memory and 168 registers a thread each); 128 tokens need
-// their accumulators' registers and take an SM alone.
+// Folding warps: four (32 weight rows each), or eight that also halve the columns, so that a lane holds at most 64 sums.
+// Up to 64 tokens two CTAs share an SM (about 110 KB of shared memory each); 128 tokens take one alone.
 template <int NT> constexpr int narrow_ctas() { return NT <= 64 ? 2 : 1; }
 template <int NT> constexpr int narrow_stages() { return NT <= 32 ? 5 : NT <= 64 ? 4 : 6; }
+template <int NT> constexpr int narrow_folders() { return NT <= 32 ? 4 : 8; }
+template <int NT> constexpr int narrow_cols() { return NT * 4 / narrow_folders<NT>(); }
+template <int NT> constexpr int narrow_threads() { return 64 + 32 * narrow_folders<NT>(); }
 
 template <int NT>
 struct __align__(1024) NarrowSmem {
   static constexpr int kStageBytes = (kBlock + NT) * kBlock;
   uint8_t tiles[narrow_stages<NT>()][kStageBytes];    // the K loop's ring, afterwards this CTA's partial sums [NT][128]
-  float factor[4][2][NT];                             // per epilogue warp: sa * sb of a K block
+  float factor[narrow_folders<NT>()][2][narrow_cols<NT>()];      // sa * sb of a K block
   GroupTable groups;
   uint64_t full[narrow_stages<NT>()], empty[narrow_stages<NT>()], tmem_full[kNarrowBufs], tmem_empty[kNarrowBufs];
   uint32_t tmem_base;
   volatile int abort_flag;
 };
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
 
@@ -375,24 +402,31 @@ __device__ __forceinline__ void store_one(const Params& p, int64_t row, int64_t 
   }
 }
 
-// `COLS` (16, or a multiple of 32) consecutive tensor-memory columns of this lane's row
-template <int COLS>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[COLS]) {
-  if constexpr (COLS == 16) {
-    tc05::tmem_ld_32x16(taddr, r);
-    tc05::tmem_ld_wait(r);
-  } else {
-#pragma unroll
-    for (int c = 0; c < COLS; c += 32) tc05::tmem_ld_32x32(taddr + c, *reinterpret_cast<uint32_t(*)[32]>(&r[c]));
-#pragma unroll
-    for (int c = 0; c < COLS; c += 32) tc05::tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(&r[c]));
+// four consecutive outputs of a row
+__device__ __forceinline__ void store_four(const Params& p, int64_t row, int64_t n, float4 v) {
+  const int64_t off = row * p.ld_out + n;
+  if (p.out_kind != AMCT_GEMM_OUT_F32 && n + 3 < p.n && ((reinterpret_cast<uintptr_t>(p.out) + 2 * off) & 7) == 0) {
+    uint2 h;
+    if (p.out_kind == AMCT_GEMM_OUT_BF16) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+      h = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+      const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+      h = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + off) = h;
+    return;
   }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < p.n) store_one(p, row, n + i, f[i]);
 }
 
 // Grid: splits CTAs (one cluster) for each tile.  CTA `rank` of a cluster takes the K blocks
 // [rank * num_kb / splits, (rank + 1) * num_kb / splits).
 template <int NT, bool GROUPED>
-__global__ void __launch_bounds__(kNarrowThreads, narrow_ctas<NT>())
+__global__ void __launch_bounds__(narrow_threads<NT>(), narrow_ctas<NT>())
 gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x, Params p, int splits) {
   constexpr int kStages = narrow_stages<NT>();
   constexpr uint32_t kTmemCols = NT * kNarrowBufs < 32 ? 32 : NT * kNarrowBufs;
@@ -402,27 +436,27 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
   const uint32_t rank = splits > 1 ? tc05::cluster_ctarank() : 0;
   const int num_kb_all = (int)((p.k + kBlock - 1) / kBlock);
   const int kb_lo = (int)((int64_t)num_kb_all * rank / splits), kb_hi = (int)((int64_t)num_kb_all * (rank + 1) / splits);
-  const int64_t tiles_n = (p.n + kBlock - 1) / kBlock;
-  const int64_t tile = blockIdx.x / splits;
+  const uint32_t tiles_n = (uint32_t)((p.n + kBlock - 1) / kBlock);
+  const uint32_t tile = blockIdx.x / (uint32_t)splits;
 
   Tile t;
   if (GROUPED) {
-    build_groups<kNarrowThreads, NT>(p, s.groups);
-    if (tile >= (int64_t)s.groups.first[p.experts] * tiles_n) return;      // the whole cluster leaves
+    build_groups<narrow_threads<NT>(), NT>(p, s.groups);
+    if (tile >= (uint32_t)s.groups.first[p.experts] * tiles_n) return;      // the whole cluster leaves
     t = group_tile<NT>(p, s.groups, tile, tiles_n);
   } else {
-    const int64_t tiles_m = (p.m + NT - 1) / NT;
-    t.tn = tile / tiles_m;                       // row tiles fastest: they share a slice of the weight
-    t.row0 = (tile - t.tn * tiles_m) * NT;
-    t.row_end = p.m;
+    const uint32_t tiles_m = (uint32_t)((p.m + NT - 1) / NT);
+    t.tn = (int)(tile / tiles_m);                // row tiles fastest: they share a slice of the weight
+    t.row0 = (int)(tile - (uint32_t)t.tn * tiles_m) * NT;
+    t.row_end = (int)p.m;
     t.expert = 0;
   }
-  const int64_t n0 = t.tn * kBlock;
+  const int64_t n0 = (int64_t)t.tn * kBlock;
 
   if (threadIdx.x == 0) {
     s.abort_flag = 0;
     for (int i = 0; i < kStages; ++i) { tc05::mbar_init(tc05::smem_u32(&s.full[i]), 1); tc05::mbar_init(tc05::smem_u32(&s.empty[i]), 1); }
-    for (int i = 0; i < kNarrowBufs; ++i) { tc05::mbar_init(tc05::smem_u32(&s.tmem_full[i]), 1); tc05::mbar_init(tc05::smem_u32(&s.tmem_empty[i]), 4); }
+    for (int i = 0; i < kNarrowBufs; ++i) { tc05::mbar_init(tc05::smem_u32(&s.tmem_full[i]), 1); tc05::mbar_init(tc05::smem_u32(&s.tmem_empty[i]), narrow_folders<NT>()); }
     tc05::fence_barrier_init();
     tc05::prefetch_tmap(&tma_w);
     tc05::prefetch_tmap(&tma_x);
@@ -436,21 +470,17 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
   tc05::fence_after_sync();
   const uint32_t tmem_base = s.tmem_base;
   volatile int* abort_flag = &s.abort_flag;
-  float acc[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j] = 0.f;
-
   if (warp == 0) {
     if (tc05::elect_one()) {
       uint32_t stage = 0, phase = 0;
-      const int row_w = (int)(t.expert * p.n + n0);
+      const int row_w = t.expert * (int)p.n + t.tn * kBlock;
       for (int kb = kb_lo; kb < kb_hi; ++kb) {
         if (!tc05::mbar_wait(tc05::smem_u32(&s.empty[stage]), phase ^ 1, abort_flag)) break;
         const uint32_t bar = tc05::smem_u32(&s.full[stage]);
         tc05::mbar_expect_tx(bar, NarrowSmem<NT>::kStageBytes);
         const uint32_t dst = tc05::smem_u32(&s.tiles[stage][0]);
         tc05::tma_load_2d(dst, &tma_w, bar, kb * kBlock, row_w);
-        tc05::tma_load_2d(dst + kBlock * kBlock, &tma_x, bar, kb * kBlock, (int)t.row0);
+        tc05::tma_load_2d(dst + kBlock * kBlock, &tma_x, bar, kb * kBlock, t.row0);
         if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
@@ -476,88 +506,118 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3;
-    float(&factor)[2][NT] = s.factor[warp - 2];
-    const float* sb = p.sb + t.expert * p.sb_expert + t.tn * p.sb_row;
-    constexpr int kPer = (NT + 31) / 32;         // tokens whose scale a lane fetches
-    const float* sa[kPer];
-    float next_a[kPer];
-    float next_b = __ldg(sb + (int64_t)kb_lo * p.sb_k);
+    constexpr int kCols = narrow_cols<NT>(), kPart = kCols < 32 ? kCols : 32, kPer = (kCols + 31) / 32;
+    const int quarter = warp & 3, col0 = ((warp - 2) >> 2) * kCols;
+    float(&factor)[2][kCols] = s.factor[warp - 2];
+    const float* sb = p.sb + (int64_t)t.expert * p.sb_expert + (int64_t)t.tn * p.sb_row;
+    const float* sa[kPer];                       // tokens whose scale this lane fetches
+    float a_scale[kNarrowBufs][kPer], b_scale[kNarrowBufs];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int64_t row = t.row0 + i * 32 + lane;
-      const bool in = i * 32 + lane < NT && row < t.row_end;
-      sa[i] = p.sa + (in ? row : t.row0) * p.sa_row;
-      next_a[i] = __ldg(sa[i] + (int64_t)kb_lo * p.sa_k);
+      const int c = i * 32 + lane, row = t.row0 + col0 + c;
+      sa[i] = p.sa + (int64_t)(c < kCols && row < t.row_end ? row : t.row0) * p.sa_row;
     }
-    uint32_t buf = 0, buf_phase = 0, side = 0;
-    for (int kb = kb_lo; kb < kb_hi; ++kb) {
+    // scales as many blocks ahead as there are buffers: a load from L2 takes longer than a block
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i * 32 + lane < NT) factor[side][i * 32 + lane] = __fmul_rn(next_a[i], next_b);
-      __syncwarp();                              // also: every lane has left the other side, which is written next
-      if (kb + 1 < kb_hi) {
-        next_b = __ldg(sb + (int64_t)(kb + 1) * p.sb_k);
+    for (int u = 0; u < kNarrowBufs; ++u) {
+      const int64_t kb = kb_lo + u < kb_hi ? kb_lo + u : kb_lo;
+      b_scale[u] = __ldg(sb + kb * p.sb_k);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) next_a[i] = __ldg(sa[i] + (int64_t)(kb + 1) * p.sa_k);
-      }
-      if (!warp_wait(tc05::smem_u32(&s.tmem_full[buf]), buf_phase, abort_flag)) break;
-      tc05::fence_after_sync();
-      constexpr int kPart = NT < 64 ? NT : 64;   // columns held at a time
+      for (int i = 0; i < kPer; ++i) a_scale[u][i] = __ldg(sa[i] + kb * p.sa_k);
+    }
+    float acc[kCols];
 #pragma unroll
-      for (int c0 = 0; c0 < NT; c0 += kPart) {
-        uint32_t r[kPart];
-        tmem_ld_cols<kPart>(tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * NT + c0, r);
-        if (c0 + kPart == NT) {
-          tc05::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&s.tmem_empty[buf]));
+    for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+    uint32_t buf_phase = 0;
+    bool alive = true;
+    for (int base = kb_lo; base < kb_hi && alive; base += kNarrowBufs, buf_phase ^= 1) {
+#pragma unroll
+      for (int u = 0; u < kNarrowBufs; ++u) {    // u: buffer of the block
+        const int kb = base + u;
+        if (kb >= kb_hi) break;
+        float(&f_now)[kCols] = factor[u & 1];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (i * 32 + lane < kCols) f_now[i * 32 + lane] = __fmul_rn(a_scale[u][i], b_scale[u]);
+        __syncwarp();                            // also: every lane has left the other side, which is written next
+        if (kb + kNarrowBufs < kb_hi) {
+          const int64_t later = kb + kNarrowBufs;
+          b_scale[u] = __ldg(sb + later * p.sb_k);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) a_scale[u][i] = __ldg(sa[i] + later * p.sa_k);
         }
+        if (!warp_wait(tc05::smem_u32(&s.tmem_full[u]), buf_phase, abort_flag)) { alive = false; break; }
+        tc05::fence_after_sync();
 #pragma unroll
-        for (int j = 0; j < kPart; j += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(&factor[side][c0 + j]);
-          acc[c0 + j] = __fmaf_rn(__uint_as_float(r[j]), f.x, acc[c0 + j]);
-          acc[c0 + j + 1] = __fmaf_rn(__uint_as_float(r[j + 1]), f.y, acc[c0 + j + 1]);
-          acc[c0 + j + 2] = __fmaf_rn(__uint_as_float(r[j + 2]), f.z, acc[c0 + j + 2]);
-          acc[c0 + j + 3] = __fmaf_rn(__uint_as_float(r[j + 3]), f.w, acc[c0 + j + 3]);
+        for (int c0 = 0; c0 < kCols; c0 += kPart) {
+          uint32_t r[kPart];
+          const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + u * NT + col0 + c0;
+          if constexpr (kPart == 16) tc05::tmem_ld_32x16(at, r);
+          else tc05::tmem_ld_32x32(at, r);
+          float4 f[kPart / 4];                   // on their way while the tensor memory answers
+#pragma unroll
+          for (int j = 0; j < kPart / 4; ++j) f[j] = *reinterpret_cast<const float4*>(&f_now[c0 + 4 * j]);
+          tc05::tmem_ld_wait(r);
+          if (c0 + kPart == kCols) {
+            tc05::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&s.tmem_empty[u]));
+          }
+#pragma unroll
+          for (int j = 0; j < kPart / 4; ++j) {
+            acc[c0 + 4 * j] = __fmaf_rn(__uint_as_float(r[4 * j]), f[j].x, acc[c0 + 4 * j]);
+            acc[c0 + 4 * j + 1] = __fmaf_rn(__uint_as_float(r[4 * j + 1]), f[j].y, acc[c0 + 4 * j + 1]);
+            acc[c0 + 4 * j + 2] = __fmaf_rn(__uint_as_float(r[4 * j + 2]), f[j].z, acc[c0 + 4 * j + 2]);
+            acc[c0 + 4 * j + 3] = __fmaf_rn(__uint_as_float(r[4 * j + 3]), f[j].w, acc[c0 + 4 * j + 3]);
+          }
         }
       }
-      side ^= 1;
-      if (++buf == kNarrowBufs) { buf = 0; buf_phase ^= 1; }
     }
-    const int64_t n = n0 + quarter * 32 + lane;
-    if (splits == 1) {
-      if (n < p.n && !*abort_flag) {
-        const float b = bias_at(p, n);
+    // Every copy and every MMA of this CTA has completed (the last tensor-memory buffer was full): the ring is free.  The
+    // sums turn around in it, so that a warp stores 128 consecutive outputs of a token.
+    float* partial = reinterpret_cast<float*>(&s.tiles[0][0]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (t.row0 + j < t.row_end) store_one(p, t.row0 + j, n, __fadd_rn(acc[j], b));
-      }
-    } else {
-      // every copy and every MMA of this CTA has completed (the last tensor-memory buffer is full): the ring is free
-      float* partial = reinterpret_cast<float*>(&s.tiles[0][0]);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) partial[j * kBlock + quarter * 32 + lane] = acc[j];
-    }
+    for (int j = 0; j < kCols; ++j) partial[(col0 + j) * kBlock + quarter * 32 + lane] = acc[j];
   }
 
+  __syncthreads();
   if (splits > 1) {
-    __syncwarp();
     tc05::cluster_arrive();
     tc05::cluster_wait();
-    if (warp >= 2 && !*abort_flag) {
-      const int local = (warp & 3) * 32 + lane;
-      const int64_t n = n0 + local;
-      const uint32_t mine = tc05::smem_u32(&s.tiles[0][0]) + local * 4;
-      const float b = n < p.n ? bias_at(p, n) : 0.f;
-      // column j belongs to CTA j % splits; the partial sums are added in rank order
-      for (int j = (int)rank; j < NT; j += splits) {
-        if (t.row0 + j >= t.row_end) break;
-        float sum = 0.f;
-        for (int q = 0; q < splits; ++q) sum = __fadd_rn(sum, ld_cluster(tc05::map_to_cta(mine + j * kBlock * 4, q)));
-        if (n < p.n) store_one(p, t.row0 + j, n, __fadd_rn(sum, b));
+  }
+  if (warp >= 2 && !*abort_flag) {
+    // Column j belongs to CTA j % splits, and there to one of its folding warps; a lane takes four consecutive outputs.  All
+    // CTAs' partial sums are on their way before the first is added; they are added in rank order.
+    const int64_t n = n0 + lane * 4;
+    float b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = n + i < p.n ? bias_at(p, n + i) : 0.f;
+    const uint32_t mine = tc05::smem_u32(&s.tiles[0][0]) + lane * 16;
+    for (int j = (int)rank + (warp - 2) * splits; j < NT; j += narrow_folders<NT>() * splits) {
+      if (t.row0 + j >= t.row_end) break;
+      float4 sum;
+      if (splits == 1) {
+        sum = *reinterpret_cast<const float4*>(&s.tiles[0][0] + j * kBlock * 4 + lane * 16);
+      } else {
+        float4 part[kMaxSplits];
+#pragma unroll
+        for (int q = 0; q < kMaxSplits; ++q)
+          if (q < splits) part[q] = ld_cluster4(tc05::map_to_cta(mine + j * kBlock * 4, q));
+        sum = part[0];
+#pragma unroll
+        for (int q = 1; q < kMaxSplits; ++q) {
+          if (q < splits) {
+            sum.x = __fadd_rn(sum.x, part[q].x);
+            sum.y = __fadd_rn(sum.y, part[q].y);
+            sum.z = __fadd_rn(sum.z, part[q].z);
+            sum.w = __fadd_rn(sum.w, part[q].w);
+          }
+        }
       }
+      store_four(p, t.row0 + j, n, make_float4(__fadd_rn(sum.x, b[0]), __fadd_rn(sum.y, b[1]), __fadd_rn(sum.z, b[2]), __fadd_rn(sum.w, b[3])));
     }
+  }
+  if (splits > 1) {
     __syncwarp();
     tc05::cluster_arrive();                      // nobody leaves while its partial sums are being read
     tc05::cluster_wait();
@@ -628,6 +688,7 @@ static int launch_wide(const void* a, const void* b, int64_t ld_a, int64_t ld_b,
   const int64_t tiles_n = (p.n + kWideN - 1) / kWideN;
   const int64_t row_tiles = (p.m + kBlock - 1) / kBlock + (GROUPED ? (p.experts < p.m ? p.experts : p.m) : 0);
   const int64_t most = row_tiles * tiles_n;
+  if (most > 0x7fffffffLL) return AMCT_ERR_UNSUPPORTED;
   gemm_fp8_wide_kernel<GROUPED><<<(unsigned)(most < sms ? most : sms), kWideThreads, smem, st>>>(ma, mb, p);
   AMCT_CHECK_LAUNCH();
   return AMCT_OK;
@@ -651,11 +712,11 @@ static int launch_narrow(const void* a, const void* b, int64_t ld_a, int64_t ld_
   const int64_t tiles = row_tiles * tiles_n;
   const int64_t num_kb = (p.k + kBlock - 1) / kBlock;
   int splits = 1;                                // K split until every SM has its CTAs, four K blocks left for each
-  while (splits < 8 && tiles * splits * 2 <= narrow_ctas<NT>() * sms && num_kb >= splits * 2 * 4) splits *= 2;
+  while (splits < kMaxSplits && tiles * splits * 2 <= narrow_ctas<NT>() * sms && num_kb >= splits * 2 * 4) splits *= 2;
   if (tiles * splits > 0x7fffffffLL) return AMCT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * splits), 1, 1);
-  cfg.blockDim = dim3(kNarrowThreads, 1, 1);
+  cfg.blockDim = dim3(narrow_threads<NT>(), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -677,12 +738,16 @@ template <bool GROUPED>
 static int launch(const void* a, const void* b, int64_t ld_a, int64_t ld_b, int64_t rows_b, const Params& p, cudaStream_t st) {
   const int sms = sm_count();
   if (sms <= 0) return AMCT_ERR_CUDA;
-  // rows that share a weight: all of them, or an expert's on average
+  // Rows that share a weight: all of them, or an expert's on average.  Up to 64 the narrow kernel is ahead whatever the
+  // weight (64 x 14336 x 4096: 20.6 us against 22.5; 48 x 4096 x 7168: 14 against 32).  Beyond, its 128-token form is ahead
+  // only while it can split K, that is while its tiles fill at most half the SMs (256 x 4096 x 7168: 26.7 us against 34.4;
+  // one split, 128 x 14336 x 4096: 28.7 against 24.8; 512 x 4096 x 7168: 43 against 35).
   const int64_t rows = GROUPED ? (p.m + p.experts - 1) / p.experts : p.m;
   if (rows <= 16) return launch_narrow<16, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
   if (rows <= 32) return launch_narrow<32, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
   if (rows <= 64) return launch_narrow<64, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
-  if (rows <= 128) return launch_narrow<128, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
+  const int64_t row_tiles = GROUPED ? (p.experts < p.m ? p.experts : p.m) + p.m / 128 : (p.m + 127) / 128;
+  if (row_tiles * ((p.n + kBlock - 1) / kBlock) * 2 <= sms) return launch_narrow<128, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
   return launch_wide<GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
 }
 
