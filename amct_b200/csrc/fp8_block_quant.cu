@@ -76,10 +76,15 @@ __device__ __forceinline__ float recip_fast(float x) {
   return r;
 #endif
 }
-// g / (1 + exp(-g)) * u
+// g / (1 + exp(-g)) * u.  The quotient is corrected once, which leaves it as good as a rounded division (a product with the
+// reciprocal is off by 20 % more on average, and that shows in how many codes fall on the other side of a tie).  exp(-g)
+// stops at 2^126, so that no step meets an infinity times zero; an infinite gate keeps the uncorrected quotient.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  const float e = exp2_fast(__fmul_rn(g, -1.44269504f));
-  return __fmul_rn(__fmul_rn(g, recip_fast(__fadd_rn(1.f, e))), u);
+  const float d = __fadd_rn(1.f, exp2_fast(fminf(__fmul_rn(g, -1.44269504f), 126.f)));
+  const float y = recip_fast(d);
+  const float q = __fmul_rn(g, y);
+  const float c = __fmaf_rn(__fmaf_rn(-d, q, g), y, q);
+  return __fmul_rn(c == c ? c : q, u);
 }
 
 // |v| as unsigned bits: ordered like the magnitudes, a NaN above everything
