@@ -26,9 +26,13 @@ def _p(t):
     return c_void_p(t.data_ptr()) if t is not None else c_void_p(0)
 
 
-def _stream():
+def _raw_stream():
     """Handle of the current device's current stream (asked directly: building a torch.cuda.Stream costs 3 us a call)."""
-    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def _stream():
+    return c_void_p(_raw_stream())
 
 
 def _need_cuda(*tensors):
@@ -942,21 +946,16 @@ def _addr(t):
     return t.data_ptr() if t is not None else 0
 
 
-def _raw_stream():
-    return _stream().value or 0
-
-
-def _on(*tensors):
+def _on(first, *others):
     """Context in which the tensors' one device is current; raises when they lie on several, or on the CPU."""
-    _need_cuda(*tensors)
-    device = None
-    for t in tensors:
-        if t is not None:
-            if device is None:
-                device = t.device
-            elif t.device != device:
-                raise _l.BackendError(f'tensors on different devices: {device} and {t.device}')
-    return _SAME if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    index = first.get_device()
+    if index < 0:
+        _need_cuda(first)
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _need_cuda(t)
+            raise _l.BackendError(f'tensors on different devices: {first.device} and {t.device}')
+    return _SAME if index < 0 or index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def _cdiv(a, b):

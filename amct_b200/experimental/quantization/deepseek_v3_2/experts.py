@@ -10,6 +10,7 @@ dequantizes -- and runs the two products of every expert on them.
 import torch
 
 from ....backend import ops as _ops
+from ....deploy_op.fp8_block_linear import KeepsBufferTypes
 
 
 class _Permute(torch.autograd.Function):
@@ -45,6 +46,11 @@ class _Unpermute(torch.autograd.Function):
 def permute_tokens(x, expert_ids, num_experts):
     """(rows, plan): rows[plan.row_map[t, j]] = x[t], sorted by expert; see ``ops.moe_permute``.  Differentiable in x
     (fp32 / fp16 / bf16)."""
+    if not (torch.is_grad_enabled() and x.requires_grad):
+        rows, _, plan = _ops.moe_permute(x, expert_ids, num_experts)
+        return rows, plan
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f'no gradient for {x.dtype}')
     rows, row_map, offsets = _Permute.apply(x, expert_ids, num_experts)
     return rows, _ops.MoePlan(row_map, offsets)
 
@@ -52,10 +58,12 @@ def permute_tokens(x, expert_ids, num_experts):
 def unpermute_tokens(rows, plan, weights=None):
     """out[t] = sum_j weights[t, j] * rows[plan.row_map[t, j]] for the plan of ``permute_tokens``; see
     ``ops.moe_unpermute``.  Differentiable in rows and weights."""
+    if not (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))):
+        return _ops.moe_unpermute(rows, plan, weights)
     return _Unpermute.apply(rows, weights, plan.row_map, plan.offsets)
 
 
-class FP8RoutedExperts(torch.nn.Module):
+class FP8RoutedExperts(KeepsBufferTypes):
     """The routed experts of one layer on a checkpoint's FP8 weights: down(silu(gate(x)) * up(x)) of every chosen
     expert, weighted and summed (``moe_infer`` of the reference with its experts' Linears in FP8; inference only).
 

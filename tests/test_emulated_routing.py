@@ -30,7 +30,9 @@ def library(tmp_path_factory):
 
 @pytest.fixture
 def on_cpu(library, monkeypatch):
-    return E.patch_ops(monkeypatch, library)
+    ops = E.patch_ops(monkeypatch, library)
+    monkeypatch.setattr(ops, '_raw_stream', lambda: 0)
+    return ops
 
 
 def test_emulated_fp8_block_quant(on_cpu):
