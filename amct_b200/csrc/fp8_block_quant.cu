@@ -41,10 +41,22 @@ __device__ __forceinline__ Raw8<T> load8(const T* src, int left) {
   return r;
 }
 
-// max|v| with NaN above everything; packed on the 16-bit types
+// The larger magnitude of two numbers, NaN if either is one; its sign means nothing.  One instruction, where the maximum
+// of an absolute value takes two.
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+#ifdef AMCT_CUDA_EMU
+  return fmax_nan(fabsf(a), fabsf(b));
+#else
+  float r;
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+#endif
+}
+
+// m and the eight magnitudes; packed on the 16-bit types
 __device__ __forceinline__ float absmax8(const Raw8<float>& r, float m) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m = fmax_nan(m, fabsf(r.v[e]));
+  for (int e = 0; e < 8; ++e) m = max_magnitude(m, r.v[e]);
   return m;
 }
 __device__ __forceinline__ float absmax8(const Raw8<__nv_bfloat16>& r, float m) {
@@ -137,7 +149,7 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], const Scale& sc) {
 template <bool VEC>
 __device__ __forceinline__ void store8(uint8_t* dst, int left, uint2 c) {
   if constexpr (VEC) {
-    if (left >= 8) *reinterpret_cast<uint2*>(dst) = c;
+    if (left >= 8) __stcs(reinterpret_cast<uint2*>(dst), c);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -182,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, kRows == 4 ? (sizeof(T) == 4 && SWIG
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[r][e] = silu_mul(ElemTraits<T>::to_f(raw[r].v[e]), ElemTraits<T>::to_f(up[r].v[e]));
-        top = fmax_nan(top, fabsf(v[r][e]));
+        top = max_magnitude(top, v[r][e]);
       }
       m[r] = abs_bits(top);
     } else {

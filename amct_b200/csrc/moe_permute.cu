@@ -96,13 +96,19 @@ __global__ void __launch_bounds__(kSortThreads) moe_count_kernel(Sort p) {
 }
 
 __global__ void __launch_bounds__(kSortThreads) moe_rank_kernel(Sort p, int chunks) {
-  __shared__ int count[kMaxExperts], base[kMaxExperts + 1], warp_total[kSortWarps];
+  __shared__ int count[kMaxExperts], ahead_of_me[kMaxExperts], base[kMaxExperts + 1], warp_total[kSortWarps];
   AMCT_DYNAMIC_SMEM(int, whist);                 // [kSortWarps][experts]: running counts of every warp
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int e = threadIdx.x; e < p.experts; e += kSortThreads) {
-    int total = 0;
-    for (int c = 0; c < chunks; ++c) total += p.counts[(int64_t)c * p.experts + e];
+    int total = 0, before = 0;
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) {
+      const int v = p.counts[(int64_t)c * p.experts + e];
+      total += v;
+      before += c < (int)blockIdx.x ? v : 0;
+    }
     count[e] = total;
+    ahead_of_me[e] = before;
   }
   __syncthreads();
   block_exclusive_scan<kSortThreads>(count, p.experts, base, warp_total);
@@ -110,11 +116,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_rank_kernel(Sort p, int chun
     for (int e = threadIdx.x; e <= p.experts; e += kSortThreads) p.offsets[e] = base[e];
     __syncthreads();
   }
-  for (int e = threadIdx.x; e < p.experts; e += kSortThreads) {
-    int before = 0;
-    for (int c = 0; c < (int)blockIdx.x; ++c) before += p.counts[(int64_t)c * p.experts + e];
-    base[e] += before;
-  }
+  for (int e = threadIdx.x; e < p.experts; e += kSortThreads) base[e] += ahead_of_me[e];
   const int64_t lo = (int64_t)blockIdx.x * p.chunk, hi = lo + p.chunk < p.n ? lo + p.chunk : p.n;
   int* mine = whist + warp * p.experts;
   for (int64_t sub = lo; sub < hi; sub += kSubChunk) {
@@ -188,7 +190,7 @@ __device__ __forceinline__ void copy_token(const Copy& c, int64_t token, const i
     const U v = __ldcs(src + i);
     for (int j = 0; j < c.topk; ++j) {
       const int p = pos[j], r = CLEAR && p < 0 ? ~p : p;
-      if (r >= 0 && r < n) reinterpret_cast<U*>(c.rows + (int64_t)r * c.ld_rows_bytes)[i] = CLEAR && p < 0 ? zero_unit<U>() : v;
+      if (r >= 0 && r < n) __stcs(reinterpret_cast<U*>(c.rows + (int64_t)r * c.ld_rows_bytes) + i, CLEAR && p < 0 ? zero_unit<U>() : v);
     }
   }
   if (c.scales && blockIdx.y == gridDim.y - 1) {
@@ -282,6 +284,18 @@ struct Combine {
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
+// rows pass through once: streaming loads and stores
+template <typename P> __device__ __forceinline__ P ld_pack(const void* p) {
+  P r;
+  if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4*>(&r) = __ldcs(reinterpret_cast<const uint4*>(p));
+  else r = *reinterpret_cast<const P*>(p);
+  return r;
+}
+template <typename P> __device__ __forceinline__ void st_pack(void* p, const P& v) {
+  if constexpr (sizeof(P) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+  else *reinterpret_cast<P*>(p) = v;
+}
+
 // acc += sum over u < U of wt[u] * rows[pos[u]], columns [V i, V i + V).  All U loads are issued before the first is used,
 // without a branch between them: an assignment without a row reads row 0 and is left out by a select.
 template <typename T, int V, int U>
@@ -291,7 +305,7 @@ __device__ __forceinline__ void combine_some(const T* rows, int64_t ld, int64_t 
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     r[u] = pos[u];
-    y[u] = *reinterpret_cast<const Pack<T, V>*>(rows + (int64_t)max(r[u], 0) * ld + i * V);
+    y[u] = ld_pack<Pack<T, V>>(rows + (int64_t)max(r[u], 0) * ld + i * V);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -339,7 +353,7 @@ __global__ void __launch_bounds__(kThreads) moe_combine_kernel(Combine p) {
     Pack<T, V> o;
 #pragma unroll
     for (int e = 0; e < V; ++e) o.v[e] = ElemTraits<T>::from_f(acc[e]);
-    *reinterpret_cast<Pack<T, V>*>(out + i * V) = o;
+    st_pack(out + i * V, o);
   }
 }
 
@@ -379,7 +393,7 @@ __device__ __forceinline__ void backward_some(const CombineBackward& p, const T*
     if (p.grad_weights) {
       Pack<T, V> y[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) y[u] = *reinterpret_cast<const Pack<T, V>*>(rows + (int64_t)max(r[u], 0) * p.ld_rows + i * V);
+      for (int u = 0; u < U; ++u) y[u] = ld_pack<Pack<T, V>>(rows + (int64_t)max(r[u], 0) * p.ld_rows + i * V);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -392,7 +406,7 @@ __device__ __forceinline__ void backward_some(const CombineBackward& p, const T*
         Pack<T, V> o;
 #pragma unroll
         for (int e = 0; e < V; ++e) o.v[e] = ElemTraits<T>::from_f(__fmul_rn(w[u], ElemTraits<T>::to_f(g.v[e])));
-        if (r[u] >= 0) *reinterpret_cast<Pack<T, V>*>(grad_rows + (int64_t)r[u] * p.ld_grad_rows + i * V) = o;
+        if (r[u] >= 0) st_pack(grad_rows + (int64_t)r[u] * p.ld_grad_rows + i * V, o);
       }
     }
   }
@@ -420,7 +434,7 @@ __device__ __forceinline__ void backward_some(const CombineBackward& p, const T*
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) moe_combine_backward_kernel(CombineBackward p) {
+__global__ void __launch_bounds__(kThreads, 4) moe_combine_backward_kernel(CombineBackward p) {
   __shared__ int pos[kMaxTopk];
   __shared__ float wt[kMaxTopk];
   __shared__ float part[kThreads / 32][8];
