@@ -161,7 +161,7 @@ constexpr int kWideN = 256, kWideStages = 4, kWideEpiWarps = 8, kWideThreads = 1
 constexpr int kWideRegsFirst = 40, kWideRegsFold = 232;
 constexpr int kWideA = kBlock * kBlock, kWideB = kWideN * kBlock, kWideStageBytes = kWideA + kWideB;
 
-constexpr int kTurnBytes = 32 * 66;      // per folding warp: 32 rows of 64 bytes, padded to an odd number of 16-bit words
+constexpr int kTurnBytes = 32 * 64;      // per folding warp: 64 bytes of 32 rows
 
 struct __align__(1024) WideSmem {
   uint8_t tiles[kWideStages][kWideStageBytes];
@@ -173,60 +173,62 @@ struct __align__(1024) WideSmem {
 };
 
 
-// A folding warp's 32 rows x 128 columns; `row` is this lane's.  Rows that begin at 16 bytes leave as vectors, a lane its own
-// row.  Others (an odd N) are turned around in shared memory, 64 bytes of every row at a time, and leave 32 consecutive
-// outputs per instruction: 2-byte stores of 32 different rows cost 2.6 x the whole kernel's time (777 x 5001 x 4000).
+// A folding warp's 32 rows x 128 columns, 64 bytes of every row at a time.  A lane holds a row, so the values turn around in
+// shared memory first and leave with neighbouring lanes on neighbouring outputs: 8 rows of 64 bytes for each instruction,
+// where a lane's own row would touch 32 lines with 16 bytes each.  Rows that do not begin at 16 bytes (an odd N) leave 32
+// consecutive outputs at a time.
 __device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int row_end, int lane, int64_t n0, float (&acc)[128], uint8_t* turn) {
-  const int row = warp_row0 + lane;
-  const int esize = p.out_kind == AMCT_GEMM_OUT_F32 ? 4 : 2;
+  const int esize = p.out_kind == AMCT_GEMM_OUT_F32 ? 4 : 2, per = 64 / esize;     // outputs of a row in 64 bytes
   uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
   const bool vectors = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(p.ld_out * esize)) & 15) == 0;
 #pragma unroll
   for (int c0 = 0; c0 < 128; c0 += 32) {
-    const int64_t left = p.n - (n0 + c0);
-    if (left <= 0) break;
+    if (n0 + c0 >= p.n) break;
     float y[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) y[j] = acc[c0 + j];
     if (p.bias_kind != AMCT_BIAS_NONE) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], j < left ? bias_at(p, n0 + c0 + j) : 0.f);
+      for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], n0 + c0 + j < p.n ? bias_at(p, n0 + c0 + j) : 0.f);
     }
-    uint32_t h[16];
-    if (esize == 2) epi_pack16(y, p.out_kind == AMCT_GEMM_OUT_BF16, h);
-    if (vectors && left >= 32) {
-      if (row < row_end) {
-        uint8_t* o = out + ((int64_t)row * p.ld_out + n0 + c0) * esize;
-        if (esize == 4) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(o + 4 * j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(o + 4 * j) = make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
-        }
-      }
-      continue;
-    }
+    uint32_t h[32];                              // the 32 outputs as they are stored: 16 or 32 words
     if (esize == 2) {
-      uint16_t* mine = reinterpret_cast<uint16_t*>(turn) + lane * 33;
+      uint32_t packed[16];
+      epi_pack16(y, p.out_kind == AMCT_GEMM_OUT_BF16, packed);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) mine[j] = (uint16_t)(h[j >> 1] >> (16 * (j & 1)));
-      __syncwarp();
-      for (int r = 0; r < 32 && warp_row0 + r < row_end; ++r)
-        if (lane < left) reinterpret_cast<uint16_t*>(out)[(int64_t)(warp_row0 + r) * p.ld_out + n0 + c0 + lane] = reinterpret_cast<const uint16_t*>(turn)[r * 33 + lane];
-      __syncwarp();
+      for (int j = 0; j < 16; ++j) h[j] = packed[j];
     } else {
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {     // 16 columns of every row
-        float* mine = reinterpret_cast<float*>(turn) + lane * 16;
+      for (int j = 0; j < 32; ++j) h[j] = __float_as_uint(y[j]);
+    }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) mine[(j + lane) & 15] = y[part * 16 + j];
-        __syncwarp();
-        const int half = lane >> 4, c = lane & 15;
-        for (int r = half; r < 32 && warp_row0 + r < row_end; r += 2)
-          if (part * 16 + c < left) reinterpret_cast<float*>(out)[(int64_t)(warp_row0 + r) * p.ld_out + n0 + c0 + part * 16 + c] = reinterpret_cast<const float*>(turn)[r * 16 + ((c + r) & 15)];
-        __syncwarp();
+    for (int part = 0; part < 2; ++part) {       // 64 bytes of every row; one part of 16-bit outputs, two of fp32
+      if (part * 16 * 4 >= 32 * esize) break;
+      const int64_t n = n0 + c0 + part * 16;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)                // chunk q of row r lies at chunk q ^ (r / 2 % 4): neither side conflicts
+        *reinterpret_cast<uint4*>(turn + lane * 64 + ((q ^ (lane >> 1)) & 3) * 16) =
+            make_uint4(h[part * 16 + 4 * q], h[part * 16 + 4 * q + 1], h[part * 16 + 4 * q + 2], h[part * 16 + 4 * q + 3]);
+      __syncwarp();
+      if (vectors && n + per <= p.n) {
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int r = it * 8 + (lane >> 2), q = lane & 3;
+          if (warp_row0 + r < row_end)
+            *reinterpret_cast<uint4*>(out + ((int64_t)(warp_row0 + r) * p.ld_out + n) * esize + q * 16) =
+                *reinterpret_cast<const uint4*>(turn + r * 64 + ((q ^ (r >> 1)) & 3) * 16);
+        }
+      } else {
+        const int step = esize == 2 ? 1 : 2, c = lane & (per - 1);     // 32 lanes: one row of 32, or two of 16
+        for (int r = lane / per; r < 32 && warp_row0 + r < row_end; r += step) {
+          if (n + c >= p.n) continue;
+          const uint8_t* from = turn + r * 64 + (((c * esize >> 4) ^ (r >> 1)) & 3) * 16 + (c * esize & 15);
+          uint8_t* to = out + ((int64_t)(warp_row0 + r) * p.ld_out + n + c) * esize;
+          if (esize == 2) *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+          else *reinterpret_cast<float*>(to) = *reinterpret_cast<const float*>(from);
+        }
       }
+      __syncwarp();
     }
   }
 }
@@ -290,16 +292,16 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         bool alive = true;
         for (uint32_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
           for (int kb = 0; kb < num_kb; ++kb) {
-            if (!tc05::mbar_wait(tc05::smem_u32(&s.tmem_empty[buf]), buf_phase ^ 1, abort_flag)) { alive = false; break; }
             if (!tc05::mbar_wait(tc05::smem_u32(&s.full[stage]), phase, abort_flag)) { alive = false; break; }
-            tc05::fence_after_sync();
             const uint32_t a0 = tc05::smem_u32(&s.tiles[stage][0]);
-            const uint32_t b0 = a0 + kWideA;
+            const uint64_t a_desc = tc05::smem_desc_sw128(a0), b_desc = tc05::smem_desc_sw128(a0 + kWideA);
+            if (!tc05::mbar_wait(tc05::smem_u32(&s.tmem_empty[buf]), buf_phase ^ 1, abort_flag)) { alive = false; break; }
+            tc05::fence_after_sync();
 #pragma unroll
-            for (int ks = 0; ks < kBlock / 32; ++ks)
-              tc05::umma_f8(tmem_base + buf * kWideN, tc05::smem_desc_sw128(a0 + ks * 32), tc05::smem_desc_sw128(b0 + ks * 32), idesc, ks > 0);
-            tc05::umma_commit(tc05::smem_u32(&s.empty[stage]));
+            for (int ks = 0; ks < kBlock / 32; ++ks)         // 32 bytes along K: 2 in the descriptor's units
+              tc05::umma_f8(tmem_base + buf * kWideN, a_desc + 2 * ks, b_desc + 2 * ks, idesc, ks > 0);
             tc05::umma_commit(tc05::smem_u32(&s.tmem_full[buf]));
+            tc05::umma_commit(tc05::smem_u32(&s.empty[stage]));
             if (++stage == kWideStages) { stage = 0; phase ^= 1; }
             if (++buf == 2) { buf = 0; buf_phase ^= 1; }
           }
@@ -310,6 +312,8 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     tc05::regs_inc<kWideRegsFold>();
     // ------------------------------------------------------------ fold and store: 32 rows x 128 columns per warp
     const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t full0 = tc05::smem_u32(&s.tmem_full[0]), empty0 = tc05::smem_u32(&s.tmem_empty[0]);
+    const uint32_t t_warp = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
     uint32_t buf = 0, buf_phase = 0;
     bool alive = true;
     for (uint32_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
@@ -322,31 +326,33 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
-      float next_a = __ldg(sa), next_b = __ldg(sb);
+      float next_a = __ldg(sa), b_32 = 0.f;      // b_32: lane l holds B's scale of block kb / 32 * 32 + l
+#pragma unroll 1
       for (int kb = 0; kb < num_kb; ++kb) {
-        const float f = __fmul_rn(next_a, next_b);
-        if (kb + 1 < num_kb) {                   // the next block's scales are on their way while this one is folded
-          next_a = __ldg(sa + (kb + 1) * p.sa_k);
-          next_b = __ldg(sb + (kb + 1) * p.sb_k);
-        }
-        if (!warp_wait(tc05::smem_u32(&s.tmem_full[buf]), buf_phase, abort_flag)) { alive = false; break; }
+        if ((kb & 31) == 0) b_32 = kb + lane < num_kb ? __ldg(sb + (kb + lane) * p.sb_k) : 0.f;
+        const float f = __fmul_rn(next_a, __shfl_sync(0xffffffffu, b_32, kb & 31));
+        sa += p.sa_k;
+        if (kb + 1 < num_kb) next_a = __ldg(sa); // on its way while this block is folded
+        if (!warp_wait(full0 + buf * 8, buf_phase, abort_flag)) { alive = false; break; }
         tc05::fence_after_sync();
-        const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * kWideN + half * 128;
-        uint32_t r[2][32];
-        tc05::tmem_ld_32x32(t_row, r[0]);
+        const uint32_t t_row = t_warp + buf * kWideN;
+        uint32_t r[2][16];
+        tc05::tmem_ld_32x16(t_row, r[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 7; ++c) {
           tc05::tmem_ld_wait(r[c & 1]);
-          if (c < 3) tc05::tmem_ld_32x32(t_row + (c + 1) * 32, r[(c + 1) & 1]);
-          else {
-            tc05::fence_before_sync();           // everything read: the buffer goes back before the last folds
-            __syncwarp();
-            if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&s.tmem_empty[buf]));
-          }
+          tc05::tmem_ld_32x16(t_row + (c + 1) * 16, r[(c + 1) & 1]);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c * 32 + j] = __fmaf_rn(__uint_as_float(r[c & 1][j]), f, acc[c * 32 + j]);
+          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = __fmaf_rn(__uint_as_float(r[c & 1][j]), f, acc[c * 16 + j]);
         }
-        if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+        tc05::tmem_ld_wait(r[1]);
+        tc05::fence_before_sync();               // everything read: the buffer goes back before the last folds
+        __syncwarp();
+        if (lane == 0) tc05::mbar_arrive(empty0 + buf * 8);
+        buf_phase ^= buf;
+        buf ^= 1;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[112 + j] = __fmaf_rn(__uint_as_float(r[1][j]), f, acc[112 + j]);
       }
       if (alive && cols_in) store_rows(p, t.row0 + quarter * 32, t.row_end, lane, n0, acc, s.turn[warp - 4]);
       __syncwarp();
