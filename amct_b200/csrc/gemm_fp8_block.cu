@@ -11,10 +11,12 @@
 //
 // Two kernels, both with a TMA producer warp, one MMA-issuing thread and epilogue warps:
 //   wide    128 rows of A x 256 columns, persistent.  A lane owns a row, so sa * sb is one number per K block and the fold
-//           is one FMA per element: 128 x 256 FMAs and as many tensor-memory reads against 512 cycles of MMA.
+//           is one FMA per element.  Bound by the operands' way into the SM, close to it by the folding's hand-over.
 //   narrow  for few rows (a decode batch): the weight is the 128-row MMA operand, 16 to 128 tokens are its columns.  Bound
 //           by the weight's bytes; K is split over a thread-block cluster whose CTAs add their partial sums through
 //           distributed shared memory in rank order, so a small weight still occupies every SM and results repeat.
+//           1 x 14336 x 4096: 15 us, of which 9 are the weight's 59 MB at the copy rate, 3 the way to the first operands
+//           and 2 the join; 128 rows on 32 experts of 4096 x 7168 (940 MB): 131 to 144 us, the copy rate.
 // Grouped: offsets [experts + 1] on the device say which rows belong to which expert.  Every CTA builds the table of
 // row tiles from them; a tile may read rows of the next expert (it never stores them).  Offsets that are out of
 // range or not ascending are clamped to a running maximum within [0, rows]: no access depends on their values.
@@ -155,8 +157,17 @@ __device__ __forceinline__ float bias_at(const Params& p, int64_t n) {
 
 // ---------------------------------------------------------------------------------------------- wide kernel
 // Three warpgroups: TMA and MMA warps in the first (two of its warps idle), eight folding warps in the others.  The launch
-// gives every thread 168 registers; the first group hands back all but 40, the folding groups take 232: 128 sums, two
-// 32-column loads in flight, no spills (40 + 2 x 232 = 3 x 168).
+// gives every thread 168 registers; the first group hands back all but 40, the folding groups take 232 (40 + 2 x 232 =
+// 3 x 168): 128 sums and two 16-column loads without a spill.
+//
+// What bounds it: 48 KB of operands for each K block, 64 bytes a cycle into an SM: 769 cycles (measured with the folding
+// left out; the block's MMAs alone take 520).  With the folding it is 880: a buffer's round -- MMAs until seen done 740,
+// loads 250, hand-over 250, for two buffers -- is close behind.  8192 x 8192 x 8192 back to back: 556 us = 1.98 PFLOP/s at
+// 1.43 GHz (the board's power limit); 8192 x 7168 x 8192 from cool: 434 us = 2.2 PFLOP/s.
+// Measured and left out: CTA pairs (32 KB for each block, but the hand-over crosses CTAs: 1 % faster at the largest size,
+// 15 to 80 % slower at 4096 x 7168 x 2048, 777 x 5120 x 4096 and for experts with 500 rows); sixteen folding warps (20 %
+// slower); paired FMAs (fma.rn.f32x2, 1.6 times the time); scales staged by a warp of their own (10 % slower); unrolling
+// the K loop by two (20 % slower: the folding code outgrows the instruction cache); one lane polling for its warp (25 %).
 constexpr int kWideN = 256, kWideStages = 4, kWideEpiWarps = 8, kWideThreads = 128 + 32 * kWideEpiWarps;
 constexpr int kWideRegsFirst = 40, kWideRegsFold = 232;
 constexpr int kWideA = kBlock * kBlock, kWideB = kWideN * kBlock, kWideStageBytes = kWideA + kWideB;

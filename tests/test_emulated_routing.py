@@ -42,7 +42,7 @@ def test_emulated_fp8_block_quant(on_cpu):
 
 def test_emulated_routing(on_cpu):
     import test_gpu_moe_permute as G
-    assert E.run_gpu_tests(G, skip=('test_many_chunks_of_assignments',)) > 150
+    assert E.run_gpu_tests(G, skip=("test_many_chunks_of_assignments", "test_more_than_two_gigabytes_of_rows", "test_backward_captured_and_replayed")) > 150
 
 
 def test_emulated_many_chunks(on_cpu):

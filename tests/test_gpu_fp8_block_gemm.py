@@ -295,3 +295,34 @@ def test_status_word_stays_clear():
     ops().gemm_fp8_block(a, a_scale, b, b_scale, status=word)
     ops().raise_if_timed_out(word)
     assert int(word) == 0
+
+
+def test_more_than_two_thousand_million_outputs():
+    """Output addresses beyond 32 bits: the last rows of a 70000 x 32768 result."""
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    m, n, k = 70000, 32768, 128
+    a = torch.randint(0, 2, (m, k), generator=gen, device='cuda').float().to(F8)
+    b = torch.randint(0, 2, (n, k), generator=gen, device='cuda').float().to(F8)
+    a_scale, b_scale = torch.ones(m, 1).cuda(), torch.ones(n // 128, 1).cuda()
+    got = ops().gemm_fp8_block(a, a_scale, b, b_scale)
+    for r in (0, m // 2, m - 1):
+        assert torch.equal(got[r].float(), b.float() @ a[r].float())
+
+
+@pytest.mark.parametrize('rows', [60, 2000])
+def test_grouped_captured_and_replayed_with_other_offsets(rows):
+    a, a_scale, b, b_scale = cuda(*grouped_operands(rows, 4, 130, 256, 5))
+    at = torch.tensor([0, 10, 20, 30, 60], dtype=torch.int32).cuda()
+    out = torch.zeros(rows, 130, dtype=torch.bfloat16).cuda()
+    ops().gemm_fp8_block_grouped(a, a_scale, at, b, b_scale, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops().gemm_fp8_block_grouped(a, a_scale, at, b, b_scale, out=out)
+    for cuts in ([0, 0, 50, 50, rows], [5, 6, 7, 40, 59]):
+        at.copy_(torch.tensor(cuts, dtype=torch.int32))
+        out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ops().gemm_fp8_block_grouped(a, a_scale, at, b, b_scale, out=torch.full_like(out, 7))
+        assert torch.equal(out, want)

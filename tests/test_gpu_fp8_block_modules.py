@@ -65,7 +65,7 @@ def test_checkpoint_linear_agrees_with_its_dequantized_weight():
     assert bool(((got - want).abs() <= size * (2.0 ** -13 + 2.0 ** -24) + want.abs() * half_step(torch.bfloat16) * 1.01).all())
 
 
-@pytest.mark.parametrize('tokens', [1, 3, 40, 700])
+@pytest.mark.parametrize('tokens', [0, 1, 3, 40, 700])
 @pytest.mark.parametrize('index_dtype', [torch.int64, torch.int32])
 def test_routed_experts_of_a_checkpoint(tokens, index_dtype):
     """moe_infer against the chain in 64 bits.  Between the two products the kernels' fp32 sums and the exact ones may fall on

@@ -242,3 +242,49 @@ def test_gradient_shortcuts():
     x.grad = None
     y.sum().backward()
     assert torch.equal(x.grad, torch.full_like(x, 4.0))
+
+
+def test_more_than_two_gigabytes_of_rows():
+    """Row addresses beyond 32 bits, in bytes and in elements."""
+    o = ops()
+    tokens, topk, hidden = 1 << 15, 8, 16384
+    x = torch.randint(0, 256, (tokens, hidden), dtype=torch.uint8, device='cuda')
+    ids = torch.randint(0, 64, (tokens, topk), device='cuda')
+    rows, _, plan = o.moe_permute(x, ids, 64)
+    for t in (0, 1, tokens // 2, tokens - 1):
+        assert torch.equal(rows[plan.row_map[t].long()], x[t].expand(topk, hidden))
+    assert int(plan.row_map.max()) == tokens * topk - 1 and torch.equal(rows[-1], x[(plan.row_map == tokens * topk - 1).nonzero()[0, 0]])
+    y = o.moe_unpermute(rows[:, :1].expand(-1, hidden)[:, :8].to(torch.float32), plan)
+    assert torch.equal(y[:, 0], x[:, 0].float() * topk)
+
+
+def test_backward_captured_and_replayed():
+    """A training step's dispatch and combine inside a CUDA graph, replayed with other values and other routing."""
+    m = experts_module()
+    tokens, topk, experts, hidden = 30, 2, 4, 64
+    x, w = torch.zeros(tokens, hidden, device='cuda', requires_grad=True), torch.zeros(tokens, topk, device='cuda', requires_grad=True)
+    ids = torch.zeros(tokens, topk, dtype=torch.int64, device='cuda')
+    c = torch.randn(tokens, hidden, device='cuda')
+
+    def step():
+        rows, plan = m.permute_tokens(x, ids, experts)
+        return torch.autograd.grad((m.unpermute_tokens(rows, plan, w) * c).sum(), (x, w))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gx, gw = step()
+    for seed in (1, 2):
+        gen = torch.Generator().manual_seed(seed)
+        with torch.no_grad():
+            x.copy_(torch.randn(tokens, hidden, generator=gen))
+            w.copy_(torch.rand(tokens, topk, generator=gen))
+            ids.copy_(torch.randint(-1, experts, (tokens, topk), generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        want_x, want_w = step()
+        assert torch.equal(gx, want_x) and torch.equal(gw, want_w)
