@@ -14,17 +14,21 @@ from ....deploy_op.fp8_block_linear import KeepsBufferTypes
 
 
 class _Permute(torch.autograd.Function):
+    """rows alone: the plan leaves through `plan_out`, because every further output costs the backward pass a tensor of zeros
+    for its missing gradient (two launches here)."""
+
     @staticmethod
-    def forward(ctx, x, expert_ids, num_experts):
+    def forward(ctx, x, expert_ids, num_experts, plan_out):
         rows, _, plan = _ops.moe_permute(x, expert_ids, num_experts)
-        ctx.save_for_backward(*plan)
-        ctx.mark_non_differentiable(*plan)
-        return rows, plan.row_map, plan.offsets
+        ctx.save_for_backward(plan.row_map)
+        plan_out.append(plan)
+        return rows
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_rows, _row_map, _offsets):
-        return _ops.moe_unpermute(grad_rows, _ops.MoePlan(*ctx.saved_tensors)), None, None
+    def backward(ctx, grad_rows):
+        (row_map,) = ctx.saved_tensors
+        return _ops.moe_unpermute(grad_rows, _ops.MoePlan(row_map, None)), None, None, None
 
 
 class _Unpermute(torch.autograd.Function):
@@ -51,8 +55,9 @@ def permute_tokens(x, expert_ids, num_experts):
         return rows, plan
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise ValueError(f'no gradient for {x.dtype}')
-    rows, row_map, offsets = _Permute.apply(x, expert_ids, num_experts)
-    return rows, _ops.MoePlan(row_map, offsets)
+    plan_out = []
+    rows = _Permute.apply(x, expert_ids, num_experts, plan_out)
+    return rows, plan_out[0]
 
 
 def unpermute_tokens(rows, plan, weights=None):
