@@ -26,13 +26,9 @@ def _p(t):
     return c_void_p(t.data_ptr()) if t is not None else c_void_p(0)
 
 
-def _raw_stream():
-    """Handle of the current device's current stream (asked directly: building a torch.cuda.Stream costs 3 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
-
-
 def _stream():
-    return c_void_p(_raw_stream())
+    """Handle of the current device's current stream (asked directly: building a torch.cuda.Stream costs 3 us a call)."""
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _need_cuda(*tensors):
@@ -946,6 +942,11 @@ def _addr(t):
     return t.data_ptr() if t is not None else 0
 
 
+def _raw_stream():
+    """_stream() as a number, for callers that hold a CUDA tensor (CUDA is initialised)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
 def _on(first, *others):
     """Context in which the tensors' one device is current; raises when they lie on several, or on the CPU."""
     index = first.get_device()
@@ -955,7 +956,7 @@ def _on(first, *others):
         if t is not None and t.get_device() != index:
             _need_cuda(t)
             raise _l.BackendError(f'tensors on different devices: {first.device} and {t.device}')
-    return _SAME if index < 0 or index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _SAME if index < 0 or index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _cdiv(a, b):
@@ -1128,9 +1129,11 @@ MOE_FEW_ASSIGNMENTS = 1024
 
 def _strided_rows(t):
     """[R, C] with unit inner stride and rows that do not overlap (copied otherwise), and the row stride."""
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    rows, cols = t.shape
+    ld, inner = t.stride()
+    if inner != 1 or (rows > 1 and ld < cols):
+        t, ld = t.contiguous(), cols
+    return t, (ld if rows > 1 else cols)
 
 
 def moe_permute(x, expert_ids, num_experts, scales=None):
@@ -1153,10 +1156,11 @@ def moe_permute(x, expert_ids, num_experts, scales=None):
     topk = expert_ids.shape[1]
     n = tokens * topk
     with _on(x, expert_ids, scales):
-        dev = x.device
+        dev, size = x.device, x.element_size()
         x, ld_x = _strided_rows(x)
         expert_ids = expert_ids.contiguous()
-        ld_rows = _cdiv(hidden, 16) * 16 if x.element_size() == 1 else hidden
+        num_experts = int(num_experts)
+        ld_rows = _cdiv(hidden, 16) * 16 if size == 1 else hidden
         rows = torch.empty_strided((n, hidden), (ld_rows, 1), dtype=x.dtype, device=dev)
         row_map = torch.empty_strided((tokens, topk), (topk, 1), dtype=torch.int32, device=dev)
         offsets = torch.empty_strided((max(num_experts, 0) + 1,), (1,), dtype=torch.int32, device=dev)
@@ -1170,21 +1174,23 @@ def moe_permute(x, expert_ids, num_experts, scales=None):
         if n > MOE_FEW_ASSIGNMENTS:
             ws = torch.empty(max(4, L.amct_moe_permute_workspace_bytes(n, num_experts)), dtype=torch.uint8, device=dev)
         rc = L.amct_moe_permute(
-            _addr(x), x.element_size(), tokens, hidden, ld_x, _addr(expert_ids),
+            x.data_ptr(), size, tokens, hidden, ld_x, expert_ids.data_ptr(),
             1 if expert_ids.dtype == torch.int64 else 0, topk, num_experts, _addr(scales), cols,
-            scales.stride(0) if cols else 0, scales.stride(1) if cols else 0, _addr(rows), ld_rows,
-            _addr(row_scales), 1, n, _addr(row_map), _addr(offsets), _addr(ws), _raw_stream())
+            scales.stride(0) if cols else 0, scales.stride(1) if cols else 0, rows.data_ptr(), ld_rows,
+            _addr(row_scales), 1, n, row_map.data_ptr(), offsets.data_ptr(), _addr(ws), _raw_stream())
         _l.check(rc, 'amct_moe_permute')
         COUNTERS['launches'] += 1 if n <= MOE_FEW_ASSIGNMENTS else 3
     return rows, row_scales, MoePlan(row_map, offsets)
 
 
 def _check_moe_plan(rows, plan, weights):
-    if rows.dim() != 2 or plan.row_map.dim() != 2 or plan.row_map.dtype != torch.int32:
+    row_map = plan.row_map
+    if rows.dim() != 2 or row_map.dim() != 2 or row_map.dtype != torch.int32:
         raise ValueError('rows must be [R, H] and plan.row_map int32 [T, topk]')
-    if rows.shape[0] != plan.row_map.numel():
-        raise ValueError(f'rows must have one row for each of the {plan.row_map.numel()} assignments')
-    if weights is not None and (weights.shape != plan.row_map.shape or weights.dtype not in _DT):
+    shape = row_map.shape
+    if rows.shape[0] != shape[0] * shape[1]:
+        raise ValueError(f'rows must have one row for each of the {row_map.numel()} assignments')
+    if weights is not None and (weights.shape != shape or weights.dtype not in _DT):
         raise ValueError('weights must be float32 / float16 / bfloat16 of the shape of the expert ids')
 
 

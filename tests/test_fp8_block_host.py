@@ -19,6 +19,12 @@ def test_argument_types_are_the_header_s():
         assert letters == want, name
 
 
+def test_the_workspace_of_the_sort_begins_where_the_wrapper_allocates_it():
+    few, handle = ops.MOE_FEW_ASSIGNMENTS, lib.load()
+    assert handle.amct_moe_permute_workspace_bytes(few, 256) == 0
+    assert handle.amct_moe_permute_workspace_bytes(few + 1, 256) >= 4 * 256
+
+
 def test_cpu_tensors_are_refused():
     x, ids = torch.zeros(2, 128), torch.zeros(2, 1, dtype=torch.int64)
     codes, scale = O.quant_tokens(x)
