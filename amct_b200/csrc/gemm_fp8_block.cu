@@ -188,6 +188,7 @@ struct __align__(1024) WideSmem {
 // shared memory first and leave with neighbouring lanes on neighbouring outputs: 8 rows of 64 bytes for each instruction,
 // where a lane's own row would touch 32 lines with 16 bytes each.  Rows that do not begin at 16 bytes (an odd N) leave 32
 // consecutive outputs at a time.
+template <bool BIAS>
 __device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int row_end, int lane, int64_t n0, float (&acc)[128], uint8_t* turn) {
   const int esize = p.out_kind == AMCT_GEMM_OUT_F32 ? 4 : 2, per = 64 / esize;     // outputs of a row in 64 bytes
   uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
@@ -198,9 +199,10 @@ __device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int r
     float y[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) y[j] = acc[c0 + j];
-    if (p.bias_kind != AMCT_BIAS_NONE) {
+    if constexpr (BIAS) {                        // one load for each lane, handed around
+      const float b = n0 + c0 + lane < p.n ? bias_at(p, n0 + c0 + lane) : 0.f;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], n0 + c0 + j < p.n ? bias_at(p, n0 + c0 + j) : 0.f);
+      for (int j = 0; j < 32; ++j) y[j] = __fadd_rn(y[j], __shfl_sync(0xffffffffu, b, j));
     }
     uint32_t h[32];                              // the 32 outputs as they are stored: 16 or 32 words
     if (esize == 2) {
@@ -231,12 +233,19 @@ __device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int r
         }
       } else {
         const int step = esize == 2 ? 1 : 2, c = lane & (per - 1);     // 32 lanes: one row of 32, or two of 16
-        for (int r = lane / per; r < 32 && warp_row0 + r < row_end; r += step) {
-          if (n + c >= p.n) continue;
+        const bool col_in = n + c < p.n;
+        const int rows = row_end - warp_row0;
+#pragma unroll 8
+        for (int r = lane / per; r < 32; r += step) {
           const uint8_t* from = turn + r * 64 + (((c * esize >> 4) ^ (r >> 1)) & 3) * 16 + (c * esize & 15);
           uint8_t* to = out + ((int64_t)(warp_row0 + r) * p.ld_out + n + c) * esize;
-          if (esize == 2) *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
-          else *reinterpret_cast<float*>(to) = *reinterpret_cast<const float*>(from);
+          if (esize == 2) {
+            const uint16_t v = *reinterpret_cast<const uint16_t*>(from);
+            if (col_in && r < rows) *reinterpret_cast<uint16_t*>(to) = v;
+          } else {
+            const float v = *reinterpret_cast<const float*>(from);
+            if (col_in && r < rows) *reinterpret_cast<float*>(to) = v;
+          }
         }
       }
       __syncwarp();
@@ -244,7 +253,8 @@ __device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int r
   }
 }
 
-template <bool GROUPED>
+// BIAS is a parameter because its code, never run, still costs the folding loop 2 %.
+template <bool GROUPED, bool BIAS>
 __global__ void __launch_bounds__(kWideThreads, 1)
 gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -365,7 +375,7 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[112 + j] = __fmaf_rn(__uint_as_float(r[1][j]), f, acc[112 + j]);
       }
-      if (alive && cols_in) store_rows(p, t.row0 + quarter * 32, t.row_end, lane, n0, acc, s.turn[warp - 4]);
+      if (alive && cols_in) store_rows<BIAS>(p, t.row0 + quarter * 32, t.row_end, lane, n0, acc, s.turn[warp - 4]);
       __syncwarp();
     }
   }
@@ -687,7 +697,7 @@ static int sm_count() {
   return n;
 }
 
-template <bool GROUPED>
+template <bool GROUPED, bool BIAS>
 static int launch_wide(const void* a, const void* b, int64_t ld_a, int64_t ld_b, int64_t rows_b, Params p, int sms, cudaStream_t st) {
   CUtensorMap ma, mb;
   int rc = make_map(&ma, a, p.m, p.k, ld_a, kBlock);
@@ -697,7 +707,7 @@ static int launch_wide(const void* a, const void* b, int64_t ld_a, int64_t ld_b,
   const size_t smem = sizeof(WideSmem) + 1024;
   static OncePerDevice attr_set;
   if (attr_set.first() &&
-      cudaFuncSetAttribute(gemm_fp8_wide_kernel<GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      cudaFuncSetAttribute(gemm_fp8_wide_kernel<GROUPED, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return AMCT_ERR_CUDA;
   // row tiles per rasterisation group: as many as keep the group's rows of A near 32 MB, a quarter of L2
   const int64_t g = (32LL << 20) / (p.k * kBlock);
@@ -706,7 +716,7 @@ static int launch_wide(const void* a, const void* b, int64_t ld_a, int64_t ld_b,
   const int64_t row_tiles = (p.m + kBlock - 1) / kBlock + (GROUPED ? (p.experts < p.m ? p.experts : p.m) : 0);
   const int64_t most = row_tiles * tiles_n;
   if (most > 0x7fffffffLL) return AMCT_ERR_UNSUPPORTED;
-  gemm_fp8_wide_kernel<GROUPED><<<(unsigned)(most < sms ? most : sms), kWideThreads, smem, st>>>(ma, mb, p);
+  gemm_fp8_wide_kernel<GROUPED, BIAS><<<(unsigned)(most < sms ? most : sms), kWideThreads, smem, st>>>(ma, mb, p);
   AMCT_CHECK_LAUNCH();
   return AMCT_OK;
 }
@@ -765,7 +775,10 @@ static int launch(const void* a, const void* b, int64_t ld_a, int64_t ld_b, int6
   if (rows <= 64) return launch_narrow<64, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
   const int64_t row_tiles = GROUPED ? (p.experts < p.m ? p.experts : p.m) + p.m / 128 : (p.m + 127) / 128;
   if (row_tiles * ((p.n + kBlock - 1) / kBlock) * 2 <= sms) return launch_narrow<128, GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
-  return launch_wide<GROUPED>(a, b, ld_a, ld_b, rows_b, p, sms, st);
+  if constexpr (!GROUPED) {
+    if (p.bias_kind != AMCT_BIAS_NONE) return launch_wide<false, true>(a, b, ld_a, ld_b, rows_b, p, sms, st);
+  }
+  return launch_wide<GROUPED, false>(a, b, ld_a, ld_b, rows_b, p, sms, st);
 }
 
 static int check(const void* a, int64_t ld_a, const float* sa, const void* b, int64_t ld_b, const float* sb, int64_t m, int64_t n,
