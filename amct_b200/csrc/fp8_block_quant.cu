@@ -92,10 +92,11 @@ __device__ __forceinline__ float recip_fast(float x) {
 #endif
 }
 // g / (1 + exp(-g)) * u.  The quotient is corrected once, which leaves it as good as a rounded division (a product with the
-// reciprocal is off by 20 % more on average, and that shows in how many codes fall on the other side of a tie).  exp(-g)
-// stops at 2^126, so that no step meets an infinity times zero; an infinite gate keeps the uncorrected quotient.
+// reciprocal is off by 20 % more on average, and that shows in how many codes fall on the other side of a tie).  Where the
+// correction meets an infinity times zero the quotient stays as it was: the reciprocal of an exponential above 2^126 is
+// zero, and so is silu down to the lowest finite gate.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  const float d = __fadd_rn(1.f, exp2_fast(fminf(__fmul_rn(g, -1.44269504f), 126.f)));
+  const float d = __fadd_rn(1.f, exp2_fast(__fmul_rn(g, -1.44269504f)));
   const float y = recip_fast(d);
   const float q = __fmul_rn(g, y);
   const float c = __fmaf_rn(__fmaf_rn(-d, q, g), y, q);

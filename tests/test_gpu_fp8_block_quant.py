@@ -121,6 +121,29 @@ def test_swiglu(rows, k, dtype):
     assert bool(((got - q).abs() <= step / 2 * (1 + 1e-6) + off / sc + q.abs() * 2.0 ** -22).all())
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows', [1, 2500])
+def test_swiglu_gates_far_below_zero(dtype, rows):
+    """silu is below 1e-80 for gates under -200, down to the type's lowest value: codes and scales are those of gates of zero,
+    whatever the other half holds.  An infinite gate below zero is inf / inf, as in the formula."""
+    gen = torch.Generator().manual_seed(rows)
+    k = 384
+    x = torch.randn(rows, 2 * k, generator=gen).to(dtype)
+    x[:, k:] = (x[:, k:].float() * 100).to(dtype)
+    low = [torch.finfo(dtype).min, torch.finfo(dtype).min / 1024, -2000.0, -200.0]
+    zero = x.clone()
+    for i in range(0, k, 5):
+        x[:, i] = low[i % 4]
+        zero[:, i] = 0
+    codes, scale = ops().fp8_block_quant(x.cuda(), act='swiglu')
+    want_c, want_s = ops().fp8_block_quant(zero.cuda(), act='swiglu')
+    assert same_scale(scale, want_s.cpu()) and same_codes(codes, want_c.cpu())
+    x[0, 130] = -float('inf')
+    x[-1, 300] = float('inf')
+    scale = ops().fp8_block_quant(x.cuda(), act='swiglu')[1].cpu()
+    assert torch.isnan(scale[0, 1]) and torch.isinf(scale[-1, 2]) and int((~torch.isfinite(scale)).sum()) == 2
+
+
 def test_strided_and_unaligned_inputs():
     base = make(40, 900, torch.bfloat16, 4).cuda()
     for view in (base[:, 3:700], base[::2, 8:520], base[:, ::2], base.t()[:300], base[5:6, 1:130]):
