@@ -14,7 +14,7 @@
 // Tokens: 16 lanes own one block, 8 elements each; a half warp takes the same block of kRows consecutive rows, so that
 // its loads are in flight together and its scales (stored block by block) leave as neighbours.  Tiles: one CTA owns a
 // 128 x 128 tile in registers.  sizeof(T) bytes read (twice that behind SwiGLU) and 1 written per element; on 16-bit inputs
-// instructions are as much of a bound as HBM (about 11 per element, 24 behind SwiGLU).  Measured, of the copy rate: bf16
+// instructions are as much of a bound as HBM (about 11 per element, 23 behind SwiGLU).  Measured, of the copy rate: bf16
 // tokens 16384 x 7168 69 us = 0.78, bf16 SwiGLU 16384 x 2048 37 us = 0.68, bf16 tiles 28672 x 8192 127 us = 0.84, fp32
 // tokens and tiles 1.03 to 1.05; 16 x 7168: 2.1 us, a launch.
 #include <cuda_fp8.h>
