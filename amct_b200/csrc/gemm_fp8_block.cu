@@ -185,17 +185,28 @@ struct __align__(1024) WideSmem {
 
 
 // A folding warp's 32 rows x 128 columns, 64 bytes of every row at a time.  A lane holds a row, so the values turn around in
-// shared memory first and leave with neighbouring lanes on neighbouring outputs: 8 rows of 64 bytes for each instruction,
-// where a lane's own row would touch 32 lines with 16 bytes each.  Rows that do not begin at 16 bytes (an odd N) leave 32
-// consecutive outputs at a time.
+// shared memory first and leave with neighbouring lanes on neighbouring outputs, where a lane's own row would touch 32 lines
+// with 16 bytes each:
+//   rows at multiples of 16 bytes: 16 bytes to a lane, 8 rows for each instruction;
+//   others (an odd N), and the last columns: a word to a lane, 2 rows for each instruction.  16-bit rows that begin in the
+//   middle of a word are shifted by one output on their way into shared memory; their first and last output go alone.
+// What counts is instructions: single outputs, 32 to an instruction, took three times as long for 4096 x 16001 x 128 as for
+// 4096 x 16000 x 128 (140 us, 46; as it is 70, and 777 x 5001 x 4000 21.8 us, 20.8 with 5008 columns).
 template <bool BIAS>
 __device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int row_end, int lane, int64_t n0, float (&acc)[128], uint8_t* turn) {
-  const int esize = p.out_kind == AMCT_GEMM_OUT_F32 ? 4 : 2, per = 64 / esize;     // outputs of a row in 64 bytes
-  uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
-  const bool vectors = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(p.ld_out * esize)) & 15) == 0;
+  const int esize = p.out_kind == AMCT_GEMM_OUT_F32 ? 4 : 2;
+  const int rows = min(row_end - warp_row0, 32), bytes = (int)(p.n - n0 < 128 ? p.n - n0 : 128) * esize;      // what exists of them
+  const int64_t ld = p.ld_out * esize;
+  uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + warp_row0 * ld + n0 * esize;
+  const bool vectors = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)ld) & 15) == 0;
+  // rows in steps of two begin alike: `half` is the first or second half of the warp
+  const int half = lane >> 4, odd = (int)((reinterpret_cast<uintptr_t>(out) + lane * ld) >> 1 & 1);
+  const int odd_row = (int)((reinterpret_cast<uintptr_t>(out) + half * ld) >> 1 & 1);
+  const uint32_t shift = odd ? 0x5432 : 0x7654;
+  uint32_t last = 0;                             // word in front of the next
 #pragma unroll
   for (int c0 = 0; c0 < 128; c0 += 32) {
-    if (n0 + c0 >= p.n) break;
+    if (n0 + c0 > p.n) break;                    // at n0 + c0 == p.n a shifted row still has its last output to come
     float y[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) y[j] = acc[c0 + j];
@@ -208,8 +219,15 @@ __device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int r
     if (esize == 2) {
       uint32_t packed[16];
       epi_pack16(y, p.out_kind == AMCT_GEMM_OUT_BF16, packed);
+      if (vectors) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) h[j] = packed[j];
+        for (int j = 0; j < 16; ++j) h[j] = packed[j];
+      } else {
+        if (c0 == 0 && odd && lane < rows) *reinterpret_cast<uint16_t*>(out + lane * ld) = (uint16_t)packed[0];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) h[j] = __byte_perm(j ? packed[j ? j - 1 : 0] : last, packed[j], shift);
+        last = packed[15];
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < 32; ++j) h[j] = __float_as_uint(y[j]);
@@ -217,40 +235,41 @@ __device__ __forceinline__ void store_rows(const Params& p, int warp_row0, int r
 #pragma unroll
     for (int part = 0; part < 2; ++part) {       // 64 bytes of every row; one part of 16-bit outputs, two of fp32
       if (part * 16 * 4 >= 32 * esize) break;
-      const int64_t n = n0 + c0 + part * 16;
+      const int at = c0 * esize + part * 64;
 #pragma unroll
       for (int q = 0; q < 4; ++q)                // chunk q of row r lies at chunk q ^ (r / 2 % 4): neither side conflicts
         *reinterpret_cast<uint4*>(turn + lane * 64 + ((q ^ (lane >> 1)) & 3) * 16) =
             make_uint4(h[part * 16 + 4 * q], h[part * 16 + 4 * q + 1], h[part * 16 + 4 * q + 2], h[part * 16 + 4 * q + 3]);
       __syncwarp();
-      if (vectors && n + per <= p.n) {
+      if (vectors && at + 64 <= bytes) {
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
           const int r = it * 8 + (lane >> 2), q = lane & 3;
-          if (warp_row0 + r < row_end)
-            *reinterpret_cast<uint4*>(out + ((int64_t)(warp_row0 + r) * p.ld_out + n) * esize + q * 16) =
-                *reinterpret_cast<const uint4*>(turn + r * 64 + ((q ^ (r >> 1)) & 3) * 16);
+          if (r < rows) *reinterpret_cast<uint4*>(out + r * ld + at + q * 16) = *reinterpret_cast<const uint4*>(turn + r * 64 + ((q ^ (r >> 1)) & 3) * 16);
         }
       } else {
-        const int step = esize == 2 ? 1 : 2, c = lane & (per - 1);     // 32 lanes: one row of 32, or two of 16
-        const bool col_in = n + c < p.n;
-        const int rows = row_end - warp_row0;
-#pragma unroll 8
-        for (int r = lane / per; r < 32; r += step) {
-          const uint8_t* from = turn + r * 64 + (((c * esize >> 4) ^ (r >> 1)) & 3) * 16 + (c * esize & 15);
-          uint8_t* to = out + ((int64_t)(warp_row0 + r) * p.ld_out + n + c) * esize;
-          if (esize == 2) {
-            const uint16_t v = *reinterpret_cast<const uint16_t*>(from);
-            if (col_in && r < rows) *reinterpret_cast<uint16_t*>(to) = v;
-          } else {
-            const float v = *reinterpret_cast<const float*>(from);
-            if (col_in && r < rows) *reinterpret_cast<float*>(to) = v;
-          }
+        const int word = lane & 15, mine = at + word * 4 - 2 * odd_row;
+        const uint8_t* from = turn + half * 64 + (word & 3) * 4;
+        uint8_t* to = out + half * ld + mine;
+        const int whole = mine >= 0 && mine + 4 <= bytes ? rows - half : 0;     // rows whose word is this lane's to store
+        const int part_of = mine >= 0 && mine + 2 == bytes ? rows - half : 0;   // ... whose last output is in it, alone
+#pragma unroll
+        for (int it = 0; it < 16; ++it) {
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(from + it * 128 + (((word >> 2) ^ it) & 3) * 16);
+          if (it * 2 < whole) *reinterpret_cast<uint32_t*>(to) = v;
+          to += 2 * ld;
+        }
+        if (bytes < 128 * esize) {
+          to = out + half * ld + mine;
+#pragma unroll 1
+          for (int it = 0; it * 2 < part_of; ++it, to += 2 * ld)
+            *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from + it * 128 + (((word >> 2) ^ it) & 3) * 16);
         }
       }
       __syncwarp();
     }
   }
+  if (odd && !vectors && esize == 2 && bytes == 256 && lane < rows) *reinterpret_cast<uint16_t*>(out + lane * ld + 254) = (uint16_t)(last >> 16);
 }
 
 // BIAS is a parameter because its code, never run, still costs the folding loop 2 %.

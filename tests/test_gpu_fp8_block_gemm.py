@@ -119,6 +119,39 @@ def test_out_is_written_where_it_should_be_and_nowhere_else(m):
         assert bool((buf == 7).all())
 
 
+# tiles enough that the 128 x 256 kernel takes them; every remainder of columns and rows that its stores treat apart
+MANY_TILES = [(70, 9601, 256), (500, 2435, 300), (777, 1502, 1100), (1300, 900, 272), (1290, 1024, 4300), (9500, 33, 128), (4900, 160, 130),
+              (2405, 512, 640), (9473, 1, 48)]
+
+
+@pytest.mark.parametrize('m,n,k', MANY_TILES)
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize('bias_dtype', [None, torch.float16])
+def test_product_of_many_tiles(m, n, k, dtype, bias_dtype):
+    test_product(m, n, k, dtype, bias_dtype)
+
+
+@pytest.mark.parametrize('m,n,k', MANY_TILES)
+def test_whole_numbers_of_many_tiles_are_exact(m, n, k):
+    test_whole_numbers_are_exact(m, n, k)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize('n', [1, 31, 32, 33, 64, 95, 96, 97, 127, 128, 129, 160, 224, 255, 256, 257, 389])
+def test_out_of_many_tiles_is_written_where_it_should_be_and_nowhere_else(n, dtype):
+    """Rows of `out` that begin at any element and lie any distance apart."""
+    m = 9600 if n <= 128 else 4900
+    a, a_scale, b, b_scale = cuda(*operands(m, n, 128, n))
+    want = ops().gemm_fp8_block(a, a_scale, b, b_scale, out_dtype=torch.float32).to(dtype)
+    for width, first in ((n, 0), (n + 1, 0), (n + 1, 1), (n + 5, 2), (n + 8 - n % 8, 0), (n + 15 - n % 8, 3)):
+        buf = torch.full((m + 2, width), 7.0, dtype=dtype).cuda()
+        out = buf[1:-1, first:first + n]
+        ops().gemm_fp8_block(a, a_scale, b, b_scale, out=out)
+        assert torch.equal(out, want)
+        buf[1:-1, first:first + n] = 7.0
+        assert bool((buf == 7).all())
+
+
 @pytest.mark.parametrize('m', [4, 140])
 def test_nan_codes_and_scales(m):
     a, a_scale, b, b_scale = operands(m, 200, 300, 2)
