@@ -99,7 +99,7 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   const float d = __fadd_rn(1.f, exp2_fast(__fmul_rn(g, -1.44269504f)));
   const float y = recip_fast(d);
   const float q = __fmul_rn(g, y);
-  const float c = __fmaf_rn(__fmaf_rn(-d, q, g), y, q);
+  const float c = __fmaf_rn(-__fmaf_rn(d, q, -g), y, q);      // this sign of the remainder: see quotient()
   return __fmul_rn(c == c ? c : q, u);
 }
 
@@ -113,10 +113,11 @@ struct Scale {
 // v / s from y = rn(1 / s): one corrected product.  The value in front of the last rounding is within 2^-45 of the
 // quotient, so the result is the correctly rounded one unless the quotient lies that close to the middle of two fp32
 // numbers; a quotient that is exactly between two codes comes out exact.  Two FMAs less than div_by_recip: these kernels
-// are bound by instructions before they are bound by memory.
+// are bound by instructions before they are bound by memory.  The remainder is formed as s q - v: for a v of -0 the form
+// v - s q is +0 and would turn the quotient's sign.
 __device__ __forceinline__ float quotient(float v, float s, float y) {
   const float q = __fmul_rn(v, y);
-  return __fmaf_rn(__fmaf_rn(-s, q, v), y, q);
+  return __fmaf_rn(-__fmaf_rn(s, q, -v), y, q);
 }
 __device__ __forceinline__ Scale block_scale(uint32_t amax_bits, bool pow2) {
   Scale r;
