@@ -7,9 +7,11 @@
 //   code = E4M3(v / s)                     (correctly rounded quotient, then round to nearest even, saturating)
 //
 // v is the input, or silu(gate) * up of the row's two halves.  That product stays in fp32: it is rounded once, to
-// its code.  silu uses the approximate base-2 exponential and reciprocal (together a few 2^-23 relative for gates of
-// ordinary size, far inside the half step of 2^-4 that a code is rounded by; 0 for gates below -87, where |silu| < 1e-35).  An infinity makes the block's scale infinite, a NaN makes
-// it NaN; both show in whatever the block is multiplied into.
+// its code.  silu uses the hardware's base-2 exponential (2 units of 2^-23 by its documentation) with what the rounding of its
+// argument left out, and a quotient as good as a rounded division: in all 2^-22 + 6 * 2^-24 + |g| 2.8e-9 relative, far inside
+// the half step of 2^-4 that a code is rounded by; 0 where exp(-g) overflows, as in the formula (gates below -88.7, where
+// |silu| < 1e-36).  An infinity makes the block's scale infinite, a NaN makes it NaN; both show in whatever the block is
+// multiplied into.
 //
 // Tokens: 16 lanes own one block, 8 elements each; a half warp takes the same block of kRows consecutive rows, so that
 // its loads are in flight together and its scales (stored block by block) leave as neighbours.  Tiles: one CTA owns a
@@ -91,17 +93,21 @@ __device__ __forceinline__ float recip_fast(float x) {
   return r;
 #endif
 }
-// g / (1 + exp(-g)) * u.  The quotient is corrected once, which leaves it as good as a rounded division (a product with the
-// reciprocal is off by 20 % more on average, and that shows in how many codes fall on the other side of a tie).  Where the
-// correction meets an infinity times zero the quotient stays as it was: the reciprocal of an exponential above 2^126 is
-// zero, and so is silu down to the lowest finite gate.
+// g / (1 + exp(-g)) * u.  exp(-g) = 2^t (1 + r) with t = rn(-g log2(e)) and r = -g - t ln 2, what the rounding of t and of
+// log2(e) left out: without it the error grows with |g| (2^-18 at 60).  The quotient from an approximate reciprocal, with
+// its remainder added once (Markstein's correction), is as good as a rounded division; the remainder's sign: see quotient().
+// Numerator and denominator are divided by four, so that the reciprocal is normal wherever exp(-g) is finite.  NaN for
+// infinite gates and where exp(-g) overflows: silu_far.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  const float d = __fadd_rn(1.f, exp2_fast(__fmul_rn(g, -1.44269504f)));
-  const float y = recip_fast(d);
-  const float q = __fmul_rn(g, y);
-  const float c = __fmaf_rn(-__fmaf_rn(d, q, -g), y, q);      // this sign of the remainder: see quotient()
-  return __fmul_rn(c == c ? c : q, u);
+  const float t = __fmul_rn(g, -1.44269504f);
+  const float e = exp2_fast(t);
+  const float d = __fmaf_rn(__fmaf_rn(e, __fmaf_rn(t, -0.693147181f, -g), e), 0.25f, 0.25f);
+  const float y = recip_fast(d), n = __fmul_rn(g, 0.25f);
+  const float q = __fmul_rn(n, y);
+  return __fmul_rn(__fmaf_rn(-__fmaf_rn(d, q, -n), y, q), u);
 }
+// its value where that is NaN: g itself far above zero, -0 far below, NaN of a NaN and (inf / inf) of -inf
+__device__ __forceinline__ float silu_far(float g, float u) { return __fmul_rn(__fmul_rn(g, __saturatef(g)), u); }
 
 // |v| as unsigned bits: ordered like the magnitudes, a NaN above everything
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -173,7 +179,7 @@ struct Params {
 };
 
 template <typename T, bool VEC, int kRows, bool SWIGLU>
-__global__ void __launch_bounds__(kThreads, kRows == 4 ? (sizeof(T) == 4 && SWIGLU ? 2 : 4) : 8) fp8_token_kernel(Params p, uint32_t kblocks, uint32_t units) {
+__global__ void __launch_bounds__(kThreads, kRows == 4 ? (sizeof(T) == 4 && SWIGLU ? 3 : 4) : 8) fp8_token_kernel(Params p, uint32_t kblocks, uint32_t units) {
   const int lane = threadIdx.x & 15;
   const uint32_t unit = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
   const bool live = unit < units;
@@ -195,11 +201,20 @@ __global__ void __launch_bounds__(kThreads, kRows == 4 ? (sizeof(T) == 4 && SWIG
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     if constexpr (SWIGLU) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[r][e] = silu_mul(ElemTraits<T>::to_f(raw[r].v[e]), ElemTraits<T>::to_f(up[r].v[e]));
       float top = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[r][e] = silu_mul(ElemTraits<T>::to_f(raw[r].v[e]), ElemTraits<T>::to_f(up[r].v[e]));
-        top = max_magnitude(top, v[r][e]);
+      for (int e = 0; e < 8; ++e) top = max_magnitude(top, v[r][e]);
+      if (top != top) {                          // rare: loads once more rather than holding the inputs' registers for it
+        const int have = row0 + r < p.rows ? left : 0;
+        const Raw8<T> g = load8<T, VEC>(x + r * p.ld_x, have), u = load8<T, VEC>(x + r * p.ld_x + p.k, have);
+        top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (v[r][e] != v[r][e]) v[r][e] = silu_far(ElemTraits<T>::to_f(g.v[e]), ElemTraits<T>::to_f(u.v[e]));
+          top = max_magnitude(top, v[r][e]);
+        }
       }
       m[r] = abs_bits(top);
     } else {

@@ -16,5 +16,6 @@ static inline unsigned __match_any_sync(unsigned, int v) {
   return mask;
 }
 static inline int atomicAdd(int* p, int v) { return __atomic_fetch_add(p, v, __ATOMIC_SEQ_CST); }
+static inline float __saturatef(float x) { return x > 0.f ? (x < 1.f ? x : 1.f) : 0.f; }
 #define __expf(x) (std::exp((float)(x)))          // a name that the C library declares too
 static inline float __fdividef(float a, float b) { return a / b; }

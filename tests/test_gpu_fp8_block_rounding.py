@@ -1,4 +1,4 @@
-"""The E4M3 block quantizer to the last bit of a code: the sign of a zero."""
+"""The E4M3 block quantizer to the last bit of a code: the sign of a zero, and silu(g) u over the whole range of gates."""
 import pytest
 import torch
 
@@ -50,3 +50,28 @@ def test_a_zero_behind_swiglu_keeps_its_sign(rows, dtype):
     want = torch.where(torch.signbit(g) != torch.signbit(u), 0x80, 0).to(torch.uint8)
     zero = (g == 0) | (u == 0)
     assert torch.equal(bytes_of(codes)[zero], want[zero])
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows', [3, 2000])
+@pytest.mark.parametrize('low,high', [(-4.0, 4.0), (-86.9, -4.0), (-88.7, -87.1), (4.0, 200.0)])
+def test_swiglu_error_does_not_grow_with_the_gate(low, high, rows, dtype):
+    """One pair in every block, so that the block's scale is |silu(g) u| / 448.  The exponential's documented error is 2 units of
+    2^-23; six further steps (its correction, 1 + exp, quotient, its remainder's rest, times u, the scale's division) round by at
+    most 2^-24 each; the correction's ln 2 is off by 2.75e-9 of itself, which costs |g| times that.  silu's own sensitivity to
+    the exponential is at most 1."""
+    gen = torch.Generator().manual_seed(rows)
+    blocks = 24
+    g = torch.rand(rows, blocks, generator=gen) * (high - low) + low
+    u = torch.exp(torch.randn(rows, blocks, generator=gen)) * (1e4 if dtype == torch.float16 else 1e8)
+    u = u.clamp(max=6e4) if dtype == torch.float16 else u
+    g, u = g.to(dtype), u.to(dtype)
+    x = torch.zeros(rows, 2, blocks, 128, dtype=dtype)
+    at = torch.randint(0, 128, (blocks,), generator=gen)
+    x[:, 0, torch.arange(blocks), at] = g
+    x[:, 1, torch.arange(blocks), at] = u
+    _, scale = ops().fp8_block_quant(x.view(rows, -1).cuda(), act='swiglu')
+    want = (g.double() * torch.sigmoid(g.double()) * u.double()).abs() / 448
+    assert float(want.min()) > 2.0 ** -126
+    bound = 2.0 ** -22 + 6 * 2.0 ** -24 + g.double().abs() * 2.8e-9
+    assert bool(((scale.cpu().double() - want).abs() <= want * bound).all())
