@@ -8,6 +8,7 @@ checkpoint's own format -- E4M3 codes and one fp32 scale for each 128 x 128 tile
 dequantizes -- and runs the two products of every expert on them.
 """
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from ....backend import ops as _ops
 from ....deploy_op.fp8_block_linear import KeepsBufferTypes
@@ -47,9 +48,17 @@ class _Unpermute(torch.autograd.Function):
         return grad_rows, grad_weights, None, None
 
 
+def _refuse_forward_mode(name, *tensors):
+    """A dual tensor need not require a gradient: past the autograd functions its tangent would be dropped in silence."""
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f'{name} has no forward-mode derivative')
+
+
 def permute_tokens(x, expert_ids, num_experts):
     """(rows, plan): rows[plan.row_map[t, j]] = x[t], sorted by expert; see ``ops.moe_permute``.  Differentiable in x
-    (fp32 / fp16 / bf16)."""
+    (fp32 / fp16 / bf16), in reverse mode and once."""
+    _refuse_forward_mode('permute_tokens', x)
     if not (torch.is_grad_enabled() and x.requires_grad):
         rows, _, plan = _ops.moe_permute(x, expert_ids, num_experts)
         return rows, plan
@@ -62,7 +71,8 @@ def permute_tokens(x, expert_ids, num_experts):
 
 def unpermute_tokens(rows, plan, weights=None):
     """out[t] = sum_j weights[t, j] * rows[plan.row_map[t, j]] for the plan of ``permute_tokens``; see
-    ``ops.moe_unpermute``.  Differentiable in rows and weights."""
+    ``ops.moe_unpermute``.  Differentiable in rows and weights, in reverse mode and once."""
+    _refuse_forward_mode('unpermute_tokens', rows, weights)
     if not (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))):
         return _ops.moe_unpermute(rows, plan, weights)
     return _Unpermute.apply(rows, weights, plan.row_map, plan.offsets)

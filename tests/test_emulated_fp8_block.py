@@ -6,3 +6,8 @@ from test_emulated_routing import library, on_cpu  # noqa: F401  (fixtures)
 def test_emulated_rounding(on_cpu):  # noqa: F811
     import test_gpu_fp8_block_rounding as G
     assert E.run_gpu_tests(G) > 50
+
+
+def test_emulated_forward_mode(on_cpu):  # noqa: F811
+    import test_gpu_moe_forward_mode as G
+    assert E.run_gpu_tests(G) == 4
