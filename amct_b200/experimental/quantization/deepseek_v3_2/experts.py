@@ -100,9 +100,18 @@ class FP8RoutedExperts(KeepsBufferTypes):
         self.first_expert, self.pow2_scale = first_expert, pow2_scale
 
     @classmethod
-    def from_checkpoint(cls, tensors, prefix, expert_numbers, first_expert=0, pow2_scale=False, device='cuda'):
+    def from_checkpoint(cls, tensors, prefix, expert_numbers, first_expert=None, pow2_scale=False, device='cuda'):
         """From the checkpoint's tensors ``{prefix}.{e}.gate_proj.weight`` / ``.weight_scale_inv`` (and up_proj,
-        down_proj) for the given expert numbers."""
+        down_proj) for the given expert numbers, which are consecutive.  ``first_expert`` is the first of them and need not be
+        given."""
+        expert_numbers = [int(e) for e in expert_numbers]
+        if not expert_numbers or expert_numbers != list(range(expert_numbers[0], expert_numbers[0] + len(expert_numbers))):
+            raise ValueError(f'expert_numbers must be consecutive numbers, at least one, not {expert_numbers}')
+        if first_expert is None:
+            first_expert = expert_numbers[0]
+        elif first_expert != expert_numbers[0]:
+            raise ValueError(f'first_expert is {first_expert}, the first of expert_numbers {expert_numbers[0]}')
+
         def stacked(*names):
             parts = [[tensors[f'{prefix}.{e}.{n}'].to(device) for n in names] for e in expert_numbers]
             codes = [[t.view(torch.uint8) if t.element_size() == 1 else t for t in p] for p in parts]
