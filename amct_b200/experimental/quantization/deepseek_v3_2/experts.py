@@ -90,9 +90,15 @@ class FP8RoutedExperts(KeepsBufferTypes):
 
     def __init__(self, gate_up_weight, gate_up_scale, down_weight, down_scale, first_expert=0, pow2_scale=False):
         super().__init__()
-        experts, width, hidden = gate_up_weight.shape
+        experts, width, hidden = gate_up_weight.shape if gate_up_weight.dim() == 3 else (0, 1, 0)
         if width % 256 or tuple(down_weight.shape) != (experts, hidden, width // 2):
             raise ValueError('gate_up_weight must be [E, 2 I, H] with I a multiple of 128, down_weight [E, H, I]')
+        for name, codes, scale in (('gate_up', gate_up_weight, gate_up_scale), ('down', down_weight, down_scale)):
+            tiles = (experts, -(-codes.shape[1] // 128), -(-codes.shape[2] // 128))
+            if codes.dtype not in (torch.float8_e4m3fn, torch.uint8):
+                raise ValueError(f'{name}_weight must hold E4M3 codes (float8_e4m3fn or uint8), not {codes.dtype}')
+            if scale.dtype != torch.float32 or tuple(scale.shape) != tiles:
+                raise ValueError(f'{name}_scale must be float32 with one value for each 128 x 128 tile, {tiles}')
         self.register_buffer('gate_up_weight', gate_up_weight)
         self.register_buffer('gate_up_scale', gate_up_scale)
         self.register_buffer('down_weight', down_weight)

@@ -30,3 +30,27 @@ def test_first_expert_is_the_first_number(numbers):
 def test_numbers_that_cannot_be_routed_are_refused(numbers, kwargs):
     with pytest.raises(ValueError, match='expert'):
         FP8RoutedExperts.from_checkpoint(checkpoint(numbers), 'mlp', numbers, device='cpu', **kwargs)
+
+
+def parts(experts=2, hidden=256, inter=128):
+    return {'gate_up_weight': torch.zeros(experts, 2 * inter, hidden, dtype=F8), 'gate_up_scale': torch.ones(experts, 2 * inter // 128, hidden // 128),
+            'down_weight': torch.zeros(experts, hidden, inter, dtype=F8), 'down_scale': torch.ones(experts, hidden // 128, inter // 128)}
+
+
+@pytest.mark.parametrize('hidden,inter', [(256, 128), (200, 128), (130, 256)])
+def test_parts_that_fit_are_taken(hidden, inter):
+    p = parts(hidden=256, inter=inter)
+    kb = -(-hidden // 128)
+    p.update(gate_up_weight=torch.zeros(2, 2 * inter, hidden, dtype=torch.uint8), gate_up_scale=torch.ones(2, 2 * inter // 128, kb),
+             down_weight=torch.zeros(2, hidden, inter, dtype=F8), down_scale=torch.ones(2, kb, inter // 128))
+    assert FP8RoutedExperts(**p).gate_up_scale.shape == (2, 2 * inter // 128, kb)
+
+
+@pytest.mark.parametrize('name,value', [
+    ('gate_up_scale', torch.ones(2, 2, 1)), ('gate_up_scale', torch.ones(2, 1, 2)), ('gate_up_scale', torch.ones(1, 2, 2)), ('gate_up_scale', torch.ones(2, 2)),
+    ('down_scale', torch.ones(2, 2, 2)), ('down_scale', torch.ones(3, 2, 1)), ('gate_up_scale', torch.ones(2, 2, 2).half()),
+    ('down_scale', torch.ones(2, 2, 1).double()), ('gate_up_weight', torch.zeros(2, 256, 256)), ('down_weight', torch.zeros(2, 256, 128).bfloat16()),
+    ('gate_up_weight', torch.zeros(256, 256, dtype=F8)), ('down_weight', torch.zeros(2, 256, 64, dtype=F8)), ('gate_up_weight', torch.zeros(2, 200, 256, dtype=F8))])
+def test_parts_that_do_not_fit_are_refused(name, value):
+    with pytest.raises(ValueError, match='must'):
+        FP8RoutedExperts(**{**parts(), name: value})
