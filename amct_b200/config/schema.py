@@ -156,6 +156,11 @@ class QuantConfig:
         self.quant_cfg = QuantCfgField(config.get('quant_cfg', {}))
         self.algorithm = AlgorithmField(config.get('algorithm', {}), registry)
         self.skip_layers = SkipLayersField(config.get('skip_layers', []))
+        # the built-in algorithms refuse it by their combination rules; a user's own algorithm may take the type
+        if self.algorithm.name == 'hifloat8':
+            for part in ('weights_cfg', 'inputs_cfg'):
+                if self.quant_cfg.value[part].get('quant_type') == 'float8_e4m3':
+                    raise ValueError(f'Algorithm hifloat8 do not support {part} type float8_e4m3')
 
 
 # ---------------------------------------------------------------------------

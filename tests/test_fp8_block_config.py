@@ -43,3 +43,17 @@ def test_refused(field, cfg):
     with pytest.raises(ValueError, match=field):
         amct.quantize(model, cfg)
     assert type(model[0]) is torch.nn.Linear
+
+
+@pytest.mark.parametrize('algorithm', [{'hifloat8': {}}, {'minmax'}, {'gptq'}, {'awq': {'grids_num': 4}}, {'smoothquant': {'smooth_strength': 0.5}}])
+@pytest.mark.parametrize('part', ['weights', 'inputs'])
+def test_the_type_belongs_to_this_algorithm(algorithm, part):
+    """None of the other algorithms here computes float8_e4m3: asked for it, they refuse instead of computing something else."""
+    plain = 'hifloat8' if 'hifloat8' in algorithm else 'int8'
+    cfg = {'batch_num': 1, 'quant_cfg': {'weights': {'type': plain, 'symmetric': True, 'strategy': 'channel'},
+                                         'inputs': {'type': plain, 'symmetric': True, 'strategy': 'token'}}, 'algorithm': algorithm}
+    cfg['quant_cfg'][part]['type'] = 'float8_e4m3'
+    model = net().to(torch.bfloat16)
+    with pytest.raises(ValueError, match='float8_e4m3'):
+        amct.quantize(model, cfg)
+    assert type(model[0]) is torch.nn.Linear
