@@ -1194,6 +1194,13 @@ def _check_moe_plan(rows, plan, weights):
         raise ValueError('weights must be float32 / float16 / bfloat16 of the shape of the expert ids')
 
 
+def check_moe_offsets(plan):
+    """The backward pass reads the last entry of plan.offsets, the number of rows in use, as an int32 on the device."""
+    offsets = plan.offsets
+    if offsets is None or offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 2:
+        raise ValueError('plan.offsets must be int32 [E + 1]')
+
+
 def moe_unpermute(rows, plan, weights=None):
     """out[t] = sum_j weights[t, j] * rows[plan.row_map[t, j]] (fp32 sum in the order of j, rounded once to rows' dtype) over
     the assignments that have a row.  weights None: ones, the gradient of moe_permute.  Returns [T, H]."""
@@ -1219,6 +1226,7 @@ def moe_unpermute_backward(grad_out, rows, plan, weights=None, want_rows=True, w
     """(grad_rows, grad_weights) of moe_unpermute for the gradient grad_out [T, H]; what is not wanted is None.  Rows that no
     assignment has get zero gradient.  rows is needed for grad_weights only."""
     _check_moe_plan(rows, plan, weights)
+    check_moe_offsets(plan)
     tokens, topk = plan.row_map.shape
     hidden = rows.shape[1]
     want_weights = want_weights and weights is not None

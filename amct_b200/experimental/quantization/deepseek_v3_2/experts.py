@@ -75,6 +75,7 @@ def unpermute_tokens(rows, plan, weights=None):
     _refuse_forward_mode('unpermute_tokens', rows, weights)
     if not (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))):
         return _ops.moe_unpermute(rows, plan, weights)
+    _ops.check_moe_offsets(plan)
     return _Unpermute.apply(rows, weights, plan.row_map, plan.offsets)
 
 
