@@ -11,6 +11,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/amct_b200.h"
 
 #define AMCT_FLT_EPSILON 1.192092896e-7f   // amct_pytorch/quantize_op/utils.py:23
@@ -201,15 +203,17 @@ __device__ __forceinline__ void epi_pack16(const float (&y)[32], bool to_bf16, u
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // "Done once per device": kernel attributes such as the dynamic shared-memory limit belong to a device's context, so a
-// process that drives several GPUs has to set them on each.  first() returns true the first time it is called with a
-// given device current (a benign race between threads only repeats the idempotent call it guards).
+// process that drives several GPUs has to set them on each.  run(set) calls set() until it has succeeded once with a given
+// device current.  The device counts as done only behind that call: threads that get here together all make the call, which
+// is idempotent, and none of them launches ahead of it; a call that failed is made again.
 struct OncePerDevice {
-  bool done[64] = {};
-  bool first() {
+  std::atomic<bool> done[64] = {};
+  template <typename F> bool run(F set) {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;
-    if (done[dev]) return false;
-    done[dev] = true;
+    const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+    if (known && done[dev].load(std::memory_order_acquire)) return true;
+    if (set() != cudaSuccess) return false;
+    if (known) done[dev].store(true, std::memory_order_release);
     return true;
   }
 };

@@ -725,8 +725,7 @@ static int launch_wide(const void* a, const void* b, int64_t ld_a, int64_t ld_b,
   if (rc != AMCT_OK) return rc;
   const size_t smem = sizeof(WideSmem) + 1024;
   static OncePerDevice attr_set;
-  if (attr_set.first() &&
-      cudaFuncSetAttribute(gemm_fp8_wide_kernel<GROUPED, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  if (!attr_set.run([&] { return cudaFuncSetAttribute(gemm_fp8_wide_kernel<GROUPED, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }))
     return AMCT_ERR_CUDA;
   // row tiles per rasterisation group: as many as keep the group's rows of A near 32 MB, a quarter of L2
   const int64_t g = (32LL << 20) / (p.k * kBlock);
@@ -749,8 +748,7 @@ static int launch_narrow(const void* a, const void* b, int64_t ld_a, int64_t ld_
   if (rc != AMCT_OK) return rc;
   const size_t smem = sizeof(NarrowSmem<NT>) + 1024;
   static OncePerDevice attr_set;
-  if (attr_set.first() &&
-      cudaFuncSetAttribute(gemm_fp8_narrow_kernel<NT, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  if (!attr_set.run([&] { return cudaFuncSetAttribute(gemm_fp8_narrow_kernel<NT, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }))
     return AMCT_ERR_CUDA;
   const int64_t tiles_n = (p.n + kBlock - 1) / kBlock;
   // grouped: no more row tiles than this, however the rows are spread over the experts

@@ -311,9 +311,7 @@ extern "C" int amct_gemm_mx(const void* a, const void* sfa_tiled, const void* b,
   p.bias = bias; p.bias_kind = bias_kind; p.out = out; p.out_kind = out_kind; p.ld_out = ld_out; p.status = status;
   const size_t smem = sizeof(Smem) + 1024;
   static amct::OncePerDevice attr_set;
-  if (attr_set.first()) {
-    if (cudaFuncSetAttribute(gemm_mx_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return AMCT_ERR_CUDA;
-  }
+  if (!attr_set.run([&] { return cudaFuncSetAttribute(gemm_mx_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); })) return AMCT_ERR_CUDA;
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -240,12 +240,12 @@ static int make_map(CUtensorMap* map, const void* base, int esize, int64_t rows,
   return AMCT_OK;
 }
 
-// Per-device facts, looked up once per device: the SM count and whether each kernel's shared-memory attribute has
-// been raised there (the attribute belongs to the device's context, not to the process).
+// Per-device facts, looked up once per device: the SM count and whether each kernel here has had its shared-memory
+// attribute raised there (the attribute belongs to the device's context, not to the process).
 constexpr int kMaxGemmDevices = 64;
 struct DeviceFacts {
   int sms = 0;
-  bool attr_small = false, attr_large = false, attr_pair = false;
+  bool attr_small = false, attr_large = false;
 };
 static DeviceFacts g_dev[kMaxGemmDevices];
 static std::mutex g_dev_mutex;
@@ -267,14 +267,6 @@ static DeviceFacts* device_facts() {
 int gemm_cta_budget() {
   DeviceFacts* f = device_facts();
   return f ? f->sms : 1;
-}
-
-// Raises the dynamic shared-memory limit of the pair kernel once per device (used by gemm_tcgen05_pair.cu).
-bool gemm_pair_attr_needed() {
-  DeviceFacts* f = device_facts();
-  if (!f || f->attr_pair) return false;
-  f->attr_pair = true;
-  return true;
 }
 
 int launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmParams& p, cudaStream_t st);

@@ -191,7 +191,6 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
 }
 
 int gemm_cta_budget();         // gemm_tcgen05.cu: SM count of the current device
-bool gemm_pair_attr_needed();  // gemm_tcgen05.cu: true once per device
 
 static int max_pairs() {
   const int n = gemm_cta_budget() / 2;
@@ -201,10 +200,9 @@ static int max_pairs() {
 // tma_a: box of 128 rows of A; tma_b: box of 128 rows of B (half a tile).
 int launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmParams& p, cudaStream_t st) {
   const size_t smem = sizeof(PairSmem) + 1024;
-  if (gemm_pair_attr_needed()) {
-    if (cudaFuncSetAttribute(gemm_tcgen05_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-      return AMCT_ERR_CUDA;
-  }
+  static OncePerDevice attr_set;
+  if (!attr_set.run([&] { return cudaFuncSetAttribute(gemm_tcgen05_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }))
+    return AMCT_ERR_CUDA;
   const int64_t tiles = ((p.m + 2 * kBM - 1) / (2 * kBM)) * ((p.n + kPairBN - 1) / kPairBN);
   const int pairs = (int)(tiles < max_pairs() ? tiles : max_pairs());
   cudaLaunchConfig_t cfg{};

@@ -133,10 +133,8 @@ extern "C" int amct_mma_peak(int kind, int steps, int ctas, int* status, void* s
   if (kind < 0 || kind > 3 || steps < 1 || ctas < 1) return AMCT_ERR_ARG;
   const size_t smem = sizeof(amct::PeakSmem) + 1024;
   static amct::OncePerDevice attr;
-  if (attr.first()) {
-    if (cudaFuncSetAttribute(amct::mma_peak_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-      return AMCT_ERR_CUDA;
-  }
+  if (!attr.run([&] { return cudaFuncSetAttribute(amct::mma_peak_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }))
+    return AMCT_ERR_CUDA;
   amct::mma_peak_kernel<<<ctas, amct::kPeakThreads, smem, (cudaStream_t)stream>>>(kind, steps, status);
   return cudaGetLastError() == cudaSuccess ? AMCT_OK : AMCT_ERR_CUDA;
 }

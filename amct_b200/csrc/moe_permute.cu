@@ -493,10 +493,8 @@ static int run_permute(const Sort& s, const Copy& c, cudaStream_t st) {
   const int chunks = (int)sort_chunks(s.n);
   const size_t smem = (size_t)kSortWarps * s.experts * sizeof(int);
   static OncePerDevice attr_set;
-  if (attr_set.first()) {
-    if (cudaFuncSetAttribute(moe_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortWarps * kMaxExperts * (int)sizeof(int)) != cudaSuccess)
-      return AMCT_ERR_CUDA;
-  }
+  if (!attr_set.run([&] { return cudaFuncSetAttribute(moe_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortWarps * kMaxExperts * (int)sizeof(int)); }))
+    return AMCT_ERR_CUDA;
   AMCT_LAUNCH((unsigned)chunks, kSortThreads, st, (s), moe_count_kernel);
   AMCT_LAUNCH_SMEM((unsigned)chunks, kSortThreads, smem, st, (s, chunks), moe_rank_kernel);
   AMCT_LAUNCH(dim3((unsigned)c.tokens, (unsigned)gy), kThreads, st, (c, (const int*)s.row_map, (const int*)(s.offsets + s.experts), s.n), moe_copy_kernel<U>);
