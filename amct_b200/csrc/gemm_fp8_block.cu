@@ -32,6 +32,9 @@ namespace f8g {
 
 constexpr int kBlock = 128;                     // rows of an MMA tile, and bytes of K per pipeline stage
 constexpr int kMaxExperts = 1024;
+// A wait that ran out leaves NaN in every output that it leaves unknown, besides its bit in the status word: a failure shows
+// without a host read, and without a status word.
+__device__ __forceinline__ float unknown() { return __int_as_float(0x7fffffff); }
 
 struct Params {
   int64_t m, n, k;
@@ -356,7 +359,7 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     const uint32_t t_warp = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
     uint32_t buf = 0, buf_phase = 0;
     bool alive = true;
-    for (uint32_t tile = blockIdx.x; tile < num_tiles && alive; tile += gridDim.x) {
+    for (uint32_t tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
       const Tile t = GROUPED ? group_tile<kBlock>(p, s.groups, tile, tiles_n) : dense_tile<kBlock>(p, tile, tiles_m, tiles_n);
       const int row = t.row0 + quarter * 32 + lane;
       const int64_t n0 = (int64_t)t.tn * kWideN + half * 128;
@@ -368,7 +371,7 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
       float next_a = __ldg(sa), b_32 = 0.f;      // b_32: lane l holds B's scale of block kb / 32 * 32 + l
 #pragma unroll 1
-      for (int kb = 0; kb < num_kb; ++kb) {
+      for (int kb = 0; kb < num_kb && alive; ++kb) {
         if ((kb & 31) == 0) b_32 = kb + lane < num_kb ? __ldg(sb + (kb + lane) * p.sb_k) : 0.f;
         const float f = __fmul_rn(next_a, __shfl_sync(0xffffffffu, b_32, kb & 31));
         sa += p.sa_k;
@@ -394,15 +397,21 @@ gemm_fp8_wide_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[112 + j] = __fmaf_rn(__uint_as_float(r[1][j]), f, acc[112 + j]);
       }
-      if (alive && cols_in) store_rows<BIAS>(p, t.row0 + quarter * 32, t.row_end, lane, n0, acc, s.turn[warp - 4]);
+      if (!alive) {                              // a wait ran out: nothing of this tile or a later one is known
+#pragma unroll
+        for (int j = 0; j < 128; ++j) acc[j] = unknown();
+      }
+      if (cols_in) store_rows<BIAS>(p, t.row0 + quarter * 32, t.row_end, lane, n0, acc, s.turn[warp - 4]);
       __syncwarp();
     }
   }
 
   __syncthreads();
   if (*abort_flag) {
-    if (threadIdx.x == 0 && p.status) atomicOr(p.status, 2);
-    for (int i = 0; i < 2000; ++i) __nanosleep(1000);      // let copies and MMAs in flight land
+    if (warp >= 4) {                             // the warps that have registers to spare
+      if (threadIdx.x == kWideThreads - 1 && p.status) atomicOr(p.status, 2);
+      tc05::let_land();
+    }
     __syncthreads();
   }
   if (warp == 1) {
@@ -436,6 +445,11 @@ struct __align__(1024) NarrowSmem {
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ int ld_cluster1(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
 
@@ -631,9 +645,13 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
     tc05::cluster_arrive();
     tc05::cluster_wait();
   }
-  if (warp >= 2 && !*abort_flag) {
+  if (warp >= 2) {
     // Column j belongs to CTA j % splits, and there to one of its folding warps; a lane takes four consecutive outputs.  All
-    // CTAs' partial sums are on their way before the first is added; they are added in rank order.
+    // CTAs' partial sums are on their way before the first is added; they are added in rank order.  A CTA whose wait ran out
+    // has only garbage to give: lane q looks at CTA q's flag, while the sums are on their way too.
+    int failed = 0;
+    if (splits == 1) failed = *abort_flag;
+    else if (lane < splits) failed = ld_cluster1(tc05::map_to_cta(tc05::smem_u32(const_cast<const int*>(&s.abort_flag)), lane));
     const int64_t n = n0 + lane * 4;
     float b[4];
 #pragma unroll
@@ -660,6 +678,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
           }
         }
       }
+      if (__any_sync(0xffffffffu, failed)) sum = make_float4(unknown(), unknown(), unknown(), unknown());
       store_four(p, t.row0 + j, n, make_float4(__fadd_rn(sum.x, b[0]), __fadd_rn(sum.y, b[1]), __fadd_rn(sum.z, b[2]), __fadd_rn(sum.w, b[3])));
     }
   }
@@ -671,7 +690,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
   __syncthreads();
   if (*abort_flag) {
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, 2);
-    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    tc05::let_land();
     __syncthreads();
   }
   if (warp == 1) {

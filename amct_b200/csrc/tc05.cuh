@@ -49,12 +49,23 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// How a wait polls, how many polls lie between two looks at its limit, and the limit: a build that tests what happens behind
+// a wait that runs out sets them.
+#ifndef AMCT_WAIT_PTX
+#define AMCT_WAIT_PTX "mbarrier.try_wait"
+#endif
+#ifndef AMCT_WAIT_POLLS
+#define AMCT_WAIT_POLLS 256
+#endif
+#ifndef AMCT_WAIT_LIMIT_NS
+#define AMCT_WAIT_LIMIT_NS 2000000000ull           // 2 s
+#endif
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n"
       ".reg .pred p;\n"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      AMCT_WAIT_PTX ".parity.shared::cta.b64 p, [%1], %2;\n"
       "selp.u32 %0, 1, 0, p;\n"
       "}\n"
       : "=r"(ok)
@@ -63,21 +74,25 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Bounded wait: gives up after `limit_ns`, or as soon as another thread of the
+// Bounded wait: gives up after AMCT_WAIT_LIMIT_NS, or as soon as another thread of the
 // CTA has given up (abort flag in shared memory).  Returns false in that case;
 // the caller leaves its loop and the kernel tears down cleanly.
-constexpr uint64_t kWaitLimitNs = 2000000000ull;   // 2 s
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   uint32_t spins = 0;
   while (!mbar_try_wait(bar, parity)) {
-    if ((++spins & 0xff) == 0) {
+    if (++spins % AMCT_WAIT_POLLS == 0) {
       if (*abort_flag) return false;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) { *abort_flag = 1; return false; }
+      if (globaltimer_ns() - t0 >= AMCT_WAIT_LIMIT_NS) { *abort_flag = 1; return false; }
     }
   }
   return true;
+}
+
+// After a wait that ran out: some two milliseconds, in which the copies and MMAs that this CTA has in flight land.
+__device__ __forceinline__ void let_land() {
+  for (int i = 0; i < 2000; ++i) __nanosleep(1000);
 }
 
 // ---- TMA ------------------------------------------------------------------
