@@ -1027,7 +1027,7 @@ def fp8_block_quant(x, block='token', act=None, pow2_scale=False):
     return codes, scale
 
 
-def _check_fp8_operands(a, a_scale, b, b_scale):
+def _check_fp8_operands(a, a_scale, b, b_scale, status):
     if a.dtype not in _CODE_DTYPES or b.dtype not in _CODE_DTYPES:
         raise ValueError('a and b must hold E4M3 codes (float8_e4m3fn or uint8)')
     if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
@@ -1043,6 +1043,8 @@ def _check_fp8_operands(a, a_scale, b, b_scale):
         raise ValueError(f'a_scale must be [{m}, {kb}], one value for each row and 128 columns')
     if b_scale.shape != (*shape[:-2], _cdiv(shape[-2], FP8_BLOCK_SIZE), kb):
         raise ValueError(f'b_scale must have one value for each 128 x 128 tile of b {tuple(shape)}')
+    if status is not None and (status.dtype != torch.int32 or status.numel() == 0):
+        raise ValueError('status must be an int32 tensor with at least one element')
 
 
 def _fp8_out(out, out_dtype, m, n, device):
@@ -1062,7 +1064,7 @@ def gemm_fp8_block(a, a_scale, b_nk, b_scale, bias=None, out_dtype=torch.bfloat1
     unknown are NaN; `status` (int32) then has bit 1, see raise_if_timed_out."""
     if a.dim() != 2 or b_nk.dim() != 2:
         raise ValueError('a must be [M, K] and b_nk [N, K]')
-    _check_fp8_operands(a, a_scale, b_nk, b_scale)
+    _check_fp8_operands(a, a_scale, b_nk, b_scale, status)
     m, k = a.shape
     n = b_nk.shape[0]
     bk = 0
@@ -1096,7 +1098,7 @@ def gemm_fp8_block_grouped(a, a_scale, offsets, b_enk, b_scale, out_dtype=torch.
     whatever the allocation held."""
     if a.dim() != 2 or b_enk.dim() != 3:
         raise ValueError('a must be [M, K] and b_enk [E, N, K]')
-    _check_fp8_operands(a, a_scale, b_enk, b_scale)
+    _check_fp8_operands(a, a_scale, b_enk, b_scale, status)
     m, k = a.shape
     experts, n = b_enk.shape[:2]
     if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() != experts + 1:
