@@ -1188,10 +1188,10 @@ def moe_permute(x, expert_ids, num_experts, scales=None):
 
 def _check_moe_plan(rows, plan, weights):
     row_map = plan.row_map
-    if rows.dim() != 2 or row_map.dim() != 2 or row_map.dtype != torch.int32:
+    if (rows is not None and rows.dim() != 2) or row_map.dim() != 2 or row_map.dtype != torch.int32:
         raise ValueError('rows must be [R, H] and plan.row_map int32 [T, topk]')
     shape = row_map.shape
-    if rows.shape[0] != shape[0] * shape[1]:
+    if rows is not None and rows.shape[0] != shape[0] * shape[1]:
         raise ValueError(f'rows must have one row for each of the {row_map.numel()} assignments')
     if weights is not None and (weights.shape != shape or weights.dtype not in _DT):
         raise ValueError('weights must be float32 / float16 / bfloat16 of the shape of the expert ids')
@@ -1227,27 +1227,29 @@ def moe_unpermute(rows, plan, weights=None):
 
 def moe_unpermute_backward(grad_out, rows, plan, weights=None, want_rows=True, want_weights=True):
     """(grad_rows, grad_weights) of moe_unpermute for the gradient grad_out [T, H]; what is not wanted is None.  Rows that no
-    assignment has get zero gradient.  rows is needed for grad_weights only."""
+    assignment has get zero gradient.  rows is read for grad_weights only and may be None without them."""
+    want_weights = want_weights and weights is not None
+    if rows is None and want_weights:
+        raise ValueError('the gradient of the weights needs the rows')
     _check_moe_plan(rows, plan, weights)
     check_moe_offsets(plan)
     tokens, topk = plan.row_map.shape
-    hidden = rows.shape[1]
-    want_weights = want_weights and weights is not None
-    if tuple(grad_out.shape) != (tokens, hidden) or grad_out.dtype != rows.dtype:
+    hidden, dtype = (rows.shape[1], rows.dtype) if rows is not None else (grad_out.shape[-1], grad_out.dtype)
+    if tuple(grad_out.shape) != (tokens, hidden) or grad_out.dtype != dtype:
         raise ValueError(f'grad_out must be [{tokens}, {hidden}] in the dtype of rows')
     with _on(grad_out, rows, plan.row_map, plan.offsets, weights):
-        dev = rows.device
-        grad_rows = torch.empty((rows.shape[0], hidden), dtype=rows.dtype, device=dev) if want_rows else None
+        dev, n = grad_out.device, tokens * topk
+        grad_rows = torch.empty((n, hidden), dtype=dtype, device=dev) if want_rows else None
         grad_weights = torch.empty((tokens, topk), dtype=weights.dtype, device=dev) if want_weights else None
         if tokens == 0 or not (want_rows or want_weights):
             return grad_rows, grad_weights
         grad_out, ld_g = _strided_rows(grad_out)
-        rows, ld = _strided_rows(rows)
+        rows, ld = _strided_rows(rows) if want_weights else (None, hidden)
         row_map = plan.row_map.contiguous()
         weights = None if weights is None else weights.contiguous()
         used = plan.offsets[-1:]
         rc = _l.load().amct_moe_unpermute_backward(
-            _addr(grad_out), _addr(rows), _dt(rows), rows.shape[0], tokens, topk, hidden,
+            _addr(grad_out), _addr(rows), _dt(grad_out), n, tokens, topk, hidden,
             ld_g, ld, _addr(row_map), _addr(used), _addr(weights), 0 if weights is None else _dt(weights),
             _addr(grad_rows), hidden, _addr(grad_weights), _raw_stream())
         _l.check(rc, 'amct_moe_unpermute_backward')

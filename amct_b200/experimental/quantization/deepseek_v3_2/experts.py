@@ -35,7 +35,8 @@ class _Permute(torch.autograd.Function):
 class _Unpermute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, row_map, offsets):
-        ctx.save_for_backward(rows, weights, row_map, offsets)
+        # the rows are read for the weights' gradient alone
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights, row_map, offsets)
         return _ops.moe_unpermute(rows, _ops.MoePlan(row_map, offsets), weights)
 
     @staticmethod

@@ -11,3 +11,8 @@ def test_emulated_rounding(on_cpu):  # noqa: F811
 def test_emulated_forward_mode(on_cpu):  # noqa: F811
     import test_gpu_moe_forward_mode as G
     assert E.run_gpu_tests(G) == 4
+
+
+def test_emulated_saved_rows(on_cpu):  # noqa: F811
+    import test_gpu_moe_saved_rows as G
+    assert E.run_gpu_tests(G) == 4
