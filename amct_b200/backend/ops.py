@@ -980,6 +980,12 @@ def _rows16(codes):
     return out[..., :k], ld
 
 
+def fp8_code_rows(codes):
+    """E4M3 codes [.., N, K] in the layout that gemm_fp8_block and gemm_fp8_block_grouped read without a copy: the tensor itself
+    if it has it, else a copy with rows that begin at multiples of 16 bytes.  On any device."""
+    return _rows16(codes)[0].view(codes.dtype)
+
+
 def fp8_block_quant(x, block='token', act=None, pow2_scale=False):
     """E4M3 codes and fp32 scales of x, one scale for each block of 128.
 

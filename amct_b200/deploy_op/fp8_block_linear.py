@@ -5,7 +5,9 @@ from ..backend import ops
 
 class KeepsBufferTypes(torch.nn.Module):
     """Module whose buffers change their device but never their type: ``.half()`` or ``.to(torch.bfloat16)`` of the model
-    around it would turn codes into numbers and round the scales."""
+    around it would turn codes into numbers and round the scales.  The ones named in ``code_buffers`` keep the layout that the
+    products read, which copies (to another device, for instance) drop."""
+    code_buffers = ()
 
     def _apply(self, fn, recurse=True):
         before = dict(self._buffers)
@@ -14,6 +16,8 @@ class KeepsBufferTypes(torch.nn.Module):
             new = self._buffers[name]
             if old is not None and new.dtype != old.dtype:
                 self._buffers[name] = old.to(new.device)
+        for name in self.code_buffers:
+            self._buffers[name] = ops.fp8_code_rows(self._buffers[name])
         return self
 
 
@@ -29,6 +33,7 @@ class FP8BlockLinear(KeepsBufferTypes):
     powers of two (checkpoints whose config says scale_fmt ue8m0).  The reference dequantizes these weights and has no
     Linear on them.
     """
+    code_buffers = ('weight',)
 
     def __init__(self, quant_module):
         super().__init__()
@@ -39,7 +44,7 @@ class FP8BlockLinear(KeepsBufferTypes):
         n, k = weight.shape
         if tuple(scale.shape) != (-(-n // 128), -(-k // 128)):
             raise ValueError(f'weight_scale_inv must have one value for each 128 x 128 tile of the weight {tuple(weight.shape)}')
-        self.register_buffer('weight', weight.view(torch.float8_e4m3fn))
+        self.register_buffer('weight', ops.fp8_code_rows(weight.view(torch.float8_e4m3fn)))
         self.register_buffer('weight_scale_inv', scale.to(torch.float32).contiguous())
         self.register_buffer('bias', None if bias is None else bias.to(torch.float32))
         self.pow2_scale = pow2_scale

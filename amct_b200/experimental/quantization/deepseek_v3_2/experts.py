@@ -89,6 +89,7 @@ class FP8RoutedExperts(KeepsBufferTypes):
     channels ahead of both products.  ``first_expert``: number of the first expert held here; assignments to experts
     of other ranks add nothing.  ``pow2_scale``: activation scales are powers of two (checkpoints whose config says
     scale_fmt ue8m0)."""
+    code_buffers = ('gate_up_weight', 'down_weight')
 
     def __init__(self, gate_up_weight, gate_up_scale, down_weight, down_scale, first_expert=0, pow2_scale=False):
         super().__init__()
@@ -101,9 +102,9 @@ class FP8RoutedExperts(KeepsBufferTypes):
                 raise ValueError(f'{name}_weight must hold E4M3 codes (float8_e4m3fn or uint8), not {codes.dtype}')
             if scale.dtype != torch.float32 or tuple(scale.shape) != tiles:
                 raise ValueError(f'{name}_scale must be float32 with one value for each 128 x 128 tile, {tiles}')
-        self.register_buffer('gate_up_weight', gate_up_weight)
+        self.register_buffer('gate_up_weight', _ops.fp8_code_rows(gate_up_weight))
         self.register_buffer('gate_up_scale', gate_up_scale)
-        self.register_buffer('down_weight', down_weight)
+        self.register_buffer('down_weight', _ops.fp8_code_rows(down_weight))
         self.register_buffer('down_scale', down_scale)
         self.first_expert, self.pow2_scale = first_expert, pow2_scale
 
