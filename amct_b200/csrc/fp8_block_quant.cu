@@ -16,9 +16,10 @@
 // Tokens: 16 lanes own one block, 8 elements each; a half warp takes the same block of kRows consecutive rows, so that
 // its loads are in flight together and its scales (stored block by block) leave as neighbours.  Tiles: one CTA owns a
 // 128 x 128 tile in registers.  sizeof(T) bytes read (twice that behind SwiGLU) and 1 written per element; on 16-bit inputs
-// instructions are as much of a bound as HBM (about 11 per element, 23 behind SwiGLU).  Measured, of the copy rate: bf16
-// tokens 16384 x 7168 69 us = 0.78, bf16 SwiGLU 16384 x 2048 37 us = 0.68, bf16 tiles 28672 x 8192 127 us = 0.84, fp32
-// tokens and tiles 1.03 to 1.05; 16 x 7168: 2.1 us, a launch.
+// instructions are as much of a bound as HBM: counted, 15 per element of a token, 12 of a tile and 30 behind SwiGLU, which
+// keep the issue slots busy for 75, 64 and 78 % of the time, and a CTA's loads, arithmetic and stores follow one another.
+// Measured, of the copy rate: bf16 tokens 16384 x 7168 70 us = 0.77, bf16 SwiGLU 16383 x 2048 38 us = 0.68, bf16 tiles
+// 28672 x 8192 127 us = 0.84, fp32 tokens and tiles 1.03 to 1.05; 16 x 7168: 1.9 us, a launch.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -116,7 +117,7 @@ struct Scale {
   float s, recip;
   bool plain;            // no step of quotient() leaves the normal range
 };
-// v / s from y = rn(1 / s): one corrected product.  The value in front of the last rounding is within 2^-45 of the
+// v / s from y = rn(1 / s): the product, corrected by its remainder once (Markstein).  The value in front of the last rounding is within 2^-45 of the
 // quotient, so the result is the correctly rounded one unless the quotient lies that close to the middle of two fp32
 // numbers; a quotient that is exactly between two codes comes out exact.  Two FMAs less than div_by_recip: these kernels
 // are bound by instructions before they are bound by memory.  The remainder is formed as s q - v: for a v of -0 the form

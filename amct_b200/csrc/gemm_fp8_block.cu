@@ -4,9 +4,13 @@
 //
 // A [rows, K] and B [N, K] (or [experts, N, K]) are E4M3 bytes, K contiguous; sa is fp32 with one value for each row and
 // 128 columns, sb one for each 128 x 128 tile: the checkpoint format that
-// amct_pytorch/experimental/quantization/DeepSeekV3.2/deploy.py:48-90 dequantizes.  The scales are arbitrary fp32
-// numbers, so they cannot ride in the MMA (its block scales are powers of two): the tensor core sums 128 products into
-// tensor memory, and the epilogue warps fold that partial sum, times sa * sb, into fp32 registers.  A tensor-memory
+// amct_pytorch/experimental/quantization/DeepSeekV3.2/deploy.py:48-90 dequantizes.  The scales may be any fp32
+// numbers, which the MMA cannot apply (its block scales are powers of two; scales that happen to be powers of two are folded
+// like the others): the tensor core sums 128 products into tensor memory, and the epilogue warps fold that partial sum, times
+// fl(sa * sb), into fp32 registers.  A product sa * sb outside the normal range of fp32 loses bits or overflows.  Against 64
+// bits the fp32 results are within 2^-21 of the sum of magnitudes for every kind of codes tried (normal, uniform bytes, one
+// large code among small ones; K from 128 to 8192), which is what an fp32 matrix product of the same numbers has; the
+// hardware documents no bound for its 128-long sums.  A tensor-memory
 // buffer holds ONE K block; there are several, so that the MMAs of the next blocks run while a block is folded in.
 //
 // Two kernels, both with a TMA producer warp, one MMA-issuing thread and epilogue warps:
@@ -166,7 +170,8 @@ __device__ __forceinline__ float bias_at(const Params& p, int64_t n) {
 // What bounds it: 48 KB of operands for each K block, 64 bytes a cycle into an SM: 769 cycles (measured with the folding
 // left out; the block's MMAs alone take 520).  With the folding it is 880: a buffer's round -- MMAs until seen done 740,
 // loads 250, hand-over 250, for two buffers -- is close behind.  8192 x 8192 x 8192 back to back: 556 us = 1.98 PFLOP/s at
-// 1.43 GHz (the board's power limit); 8192 x 7168 x 8192 from cool: 434 us = 2.2 PFLOP/s.
+// 1.43 GHz (the board's power limit); 8192 x 7168 x 8192: 435 us = 2.2 PFLOP/s for ten in a row from cool, 507 us = 1.9 in a
+// sequence of calls.
 // Measured and left out: CTA pairs (32 KB for each block, but the hand-over crosses CTAs: 1 % faster at the largest size,
 // 15 to 80 % slower at 4096 x 7168 x 2048, 777 x 5120 x 4096 and for experts with 500 rows); sixteen folding warps (20 %
 // slower); paired FMAs (fma.rn.f32x2, 1.6 times the time); scales staged by a warp of their own (10 % slower); unrolling

@@ -363,7 +363,8 @@ int amct_fp8_block_quant(const void* x, int dtype, int64_t rows, int64_t k, int6
  * (+ bias[n]): the Linear of such a checkpoint without dequantizing it.  a [m, k] and b [n, k]: E4M3 bytes, K contiguous,
  * base addresses and leading dimensions multiples of 16 bytes, any k > 0.  a_scale (i, kb) at
  * a_scale[i * a_scale_stride_row + kb * a_scale_stride_k], b_scale likewise with i = n / 128.  Each K block's dot product is
- * accumulated on the tensor cores (tcgen05 kind::f8f6f4) and folded into fp32 sums with its scales, then rounded once.
+ * accumulated on the tensor cores (tcgen05 kind::f8f6f4) and folded into fp32 sums with its scales, then rounded once; the two
+ * scales are multiplied first, in fp32.
  * bias_kind: AMCT_BIAS_NONE / F32 / F16 / BF16; out_kind: AMCT_GEMM_OUT_F32 / F16 / BF16.  Results repeat bit for bit.
  * Bit 1 of *status: a bounded device-side wait expired; what it left unknown of out is NaN, with or without a status word. */
 int amct_gemm_fp8_block(const void* a, const float* a_scale, int64_t a_scale_stride_row, int64_t a_scale_stride_k,
