@@ -1067,8 +1067,8 @@ def gemm_fp8_block(a, a_scale, b_nk, b_scale, bias=None, out_dtype=torch.bfloat1
     """a [M, K] x b_nk [N, K] -> [M, N] for E4M3 codes (float8_e4m3fn or uint8) with a scale for each block of 128:
     a_scale fp32 [M, ceil(K / 128)], b_scale fp32 [ceil(N / 128), ceil(K / 128)], any strides.  bias [N] in fp32 / fp16 / bf16.
     fp32 accumulation, rounded once to out_dtype (fp32 results: within 2^-21 of the sum of magnitudes in all measurements, as an
-    fp32 matrix product; a_scale * b_scale outside the normal range of fp32 loses bits).  No gradient (deploy path).  Outputs that a bounded wait of the kernel leaves
-    unknown are NaN; `status` (int32) then has bit 1, see raise_if_timed_out."""
+    fp32 matrix product; a_scale * b_scale outside the normal range of fp32 loses bits).  No gradient (deploy path).  Outputs
+    that a bounded wait of the kernel leaves unknown are NaN; `status` (int32) then has bit 1, see raise_if_timed_out."""
     if a.dim() != 2 or b_nk.dim() != 2:
         raise ValueError('a must be [M, K] and b_nk [N, K]')
     _check_fp8_operands(a, a_scale, b_nk, b_scale, status)

@@ -470,6 +470,40 @@ def cases():
            lambda x: (lambda: ops.dsa_rotate_fakequant(x, symmetric=False, clip_max_sigmoid=0.9, clip_min_sigmoid=0.8)),
            dict(nbytes=65536 * 512 * 4))
 
+    # ---- FP8 with a scale for each block of 128, and tokens sorted by expert
+    for what, r, k, dt, kwargs, nbytes in (('tokens', 16384, 7168, torch.bfloat16, {}, 3), ('tokens', 16384, 7168, torch.float32, {}, 5),
+                                           ('swiglu', 16383, 2048, torch.bfloat16, {'act': 'swiglu'}, 5),
+                                           ('weight tiles', 28672, 8192, torch.bfloat16, {'block': 'tile'}, 3)):
+        yield (f'fp8_block_quant {what} [{r}x{k}] {str(dt)[6:]}', lambda r=r, k=k * (2 if 'act' in kwargs else 1), dt=dt: randn(r, k, dt),
+               lambda x, kwargs=kwargs: (lambda: ops.fp8_block_quant(x, **kwargs)), dict(nbytes=r * k * nbytes))
+    for m, n, k in ((1, 14336, 4096), (64, 14336, 4096), (512, 4096, 7168), (777, 5001, 4000), (8192, 7168, 8192)):
+        def setup_f8(m=m, n=n, k=k):
+            return (*ops.fp8_block_quant(randn(m, k, torch.bfloat16)), *ops.fp8_block_quant(randn(n, k, torch.bfloat16, 0.02), block='tile'))
+        kw = dict(nops=2 * m * n * k, peak_mult=2.0) if m > 128 else dict(nbytes=n * k + m * k + 2 * m * n)
+        yield (f'gemm_fp8_block {m}x{n}x{k} -> bf16', setup_f8, lambda t: (lambda: ops.gemm_fp8_block(*t)), kw)
+
+    def setup_f8g():
+        gen = torch.Generator(device='cuda').manual_seed(1)
+        ids = torch.rand(2047, 32, generator=gen, device='cuda').argsort(1)[:, :8]
+        codes, scale = ops.fp8_block_quant(randn(2047, 7168, torch.bfloat16))
+        rows, row_scale, plan = ops.moe_permute(codes, ids, 32, scales=scale)
+        w, ws = ops.fp8_block_quant(randn(32 * 4096, 7168, torch.bfloat16, 0.02), block='tile')
+        return rows, row_scale, plan.offsets, w.view(32, 4096, 7168), ws.view(32, 32, 56)
+    yield ('gemm_fp8_block_grouped 16376 rows, 32 experts, 4096x7168 -> bf16', setup_f8g, lambda t: (lambda: ops.gemm_fp8_block_grouped(*t)),
+           dict(nops=2 * 16376 * 4096 * 7168, peak_mult=2.0))
+
+    def setup_moe():
+        ids = torch.rand(8191, 256, device='cuda').argsort(1)[:, :8]
+        x = randn(8191, 7168, torch.bfloat16)
+        rows, _, plan = ops.moe_permute(x, ids, 256)
+        return x, ids, rows, plan, torch.rand(8191, 8, device='cuda')
+    yield ('moe_permute 8191 tokens x 8, 256 experts, 7168 bf16', setup_moe, lambda t: (lambda: ops.moe_permute(t[0], t[1], 256)),
+           dict(nbytes=8191 * 9 * 7168 * 2))
+    yield ('moe_unpermute 8191 tokens x 8, 7168 bf16', setup_moe, lambda t: (lambda: ops.moe_unpermute(t[2], t[3], t[4])),
+           dict(nbytes=8191 * 9 * 7168 * 2))
+    yield ('moe_unpermute_backward 8191 tokens x 8, 7168 bf16', setup_moe, lambda t: (lambda: ops.moe_unpermute_backward(t[0], t[2], t[3], t[4])),
+           dict(nbytes=8191 * 17 * 7168 * 2))
+
 
 def main():
     ap = argparse.ArgumentParser()
