@@ -176,6 +176,14 @@ def cpu_baseline(tokens, n_layers):
             'host_cpus': os.cpu_count()}
 
 
+def cpu_baseline_or_reason(args):
+    """The CPU baseline needs the reference package; without it the line says so and keeps what was measured."""
+    try:
+        return cpu_baseline(args.cpu_sample_tokens, args.layers)
+    except Exception as exc:                                     # noqa: BLE001 -- reported, not hidden
+        return {'unavailable': f'{type(exc).__name__}: {exc}'[:300]}
+
+
 def run_reference(args):
     """--impl reference: the reference's own CPU path on the host cores, a bounded sample per step (rank 0 only)."""
     rank = int(os.environ.get('RANK', '0'))
@@ -458,7 +466,7 @@ def main():
         'clocks': clocks,
     }
     if world == 1 and not args.no_cpu_baseline:
-        line['cpu_baseline'] = cpu_baseline(args.cpu_sample_tokens, args.layers)
+        line['cpu_baseline'] = cpu_baseline_or_reason(args)
     print(json.dumps(line), flush=True)
     if world > 1:
         dist.destroy_process_group()
